@@ -3,7 +3,7 @@
 Usage: ``python build.py [--force]``.  hipcc cross-compiles, so this runs without a GPU.
 Each ``.hip`` file is compiled to an object on its own (in parallel) and the objects are
 linked into one shared library whose only exported symbols are the ``msgl_*`` C ABI of
-``include/msgl_paged_attention.h``, ``include/msgl_radix_cache.h`` and
+``include/msgl_paged_attention.h``, ``include/msgl_mxfp4_cache.h``, ``include/msgl_radix_cache.h`` and
 ``include/msgl_state_pool.h``.  ``csrc/torch_binding.cpp`` (host code: the operators' Python call
 path) is compiled by g++ against torch's headers into ``mini_sglang_amd_kernel/_native.so``, which
 loads that library from its place beside it.
@@ -22,7 +22,8 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(LIB_DIR, "libmsgl_paged_attention.so")
 SOURCES = ["api.hip", "store_kv_cache.hip", "paged_splitkv.hip", "paged_shares.hip", "paged_prefill.hip", "paged_prefill_d256.hip",
            "build_metadata.hip", "qk_norm_rope_store.hip",
-           "gdn_state.hip", "gdn_short.hip", "gdn_chunk.hip", "gdn_long.hip", "radix_cache.hip", "state_slots.hip"]
+           "gdn_state.hip", "gdn_short.hip", "gdn_chunk.hip", "gdn_long.hip", "radix_cache.hip", "state_slots.hip",
+           "mxfp4_api.hip", "mxfp4_rows.hip", "mxfp4_norm_rope.hip", "mxfp4_attention.hip"]
 
 NATIVE_SRC = os.path.join(CSRC, "torch_binding.cpp")
 NATIVE_PATH = os.path.join(HERE, "mini_sglang_amd_kernel", "_native.so")
@@ -83,9 +84,8 @@ def build(force: bool = False, save_temps: bool = False) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
-    headers.append(os.path.join(HERE, "..", "include", "msgl_paged_attention.h"))
-    headers.append(os.path.join(HERE, "..", "include", "msgl_radix_cache.h"))
-    headers.append(os.path.join(HERE, "..", "include", "msgl_state_pool.h"))
+    include = os.path.join(HERE, "..", "include")
+    headers += [os.path.join(include, f) for f in sorted(os.listdir(include)) if f.endswith(".h")]
     todo = []
     for src in SOURCES:
         obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
@@ -99,7 +99,7 @@ def build(force: bool = False, save_temps: bool = False) -> str:
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stderr}")
-    if force or _newer([NATIVE_SRC, headers[-3]], NATIVE_PATH):
+    if force or _newer([NATIVE_SRC, *(h for h in headers if h.startswith(include))], NATIVE_PATH):
         _build_native()
     return LIB_PATH
 

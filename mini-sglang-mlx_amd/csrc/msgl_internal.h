@@ -5,6 +5,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/msgl_mxfp4_cache.h"
 #include "../../include/msgl_paged_attention.h"
 #include "../../include/msgl_state_pool.h"
 
@@ -221,6 +222,77 @@ void gdn_set_rows(int v);
 int launch_state_slots(void* base, int64_t layer_stride, int64_t slot_stride, int64_t row_bytes,
                        int64_t n_layers, int64_t num_slots, const int32_t* src, const int32_t* dst,
                        int64_t n_pairs, hipStream_t stream);
+
+// ---- pool in 4 bits (mxfp4.h) -----------------------------------------------------------
+struct Mxfp4Pool {
+  void* codes;
+  void* scales;
+  int64_t codes_stride0, scales_stride0;  // bytes
+  int64_t num_slots, n_kv, head_dim;
+};
+// mxfp4_rows.hip
+struct Mxfp4StoreArgs {
+  Mxfp4Pool pool;
+  const int32_t* indices;
+  const void* k;
+  const void* v;
+  int64_t length, k_stride0, v_stride0;  // elements
+  int32_t f16;
+};
+int launch_store_mxfp4(const Mxfp4StoreArgs& a, hipStream_t stream);
+struct Mxfp4LoadArgs {
+  Mxfp4Pool pool;
+  const int32_t* indices;
+  void* k;
+  void* v;
+  int64_t length;
+  int32_t f16;
+};
+int launch_load_mxfp4(const Mxfp4LoadArgs& a, hipStream_t stream);
+// The rows listed at positions 0 .. total_kv - 1 of kv_indices as bf16, in that order, and the numbers 0 .. total_kv - 1; under a window that
+// only reaches back (window > 0) only those near what a query of its request sees.
+struct Mxfp4UnpackArgs {
+  Mxfp4Pool pool;
+  const int32_t *kv_indptr, *kv_indices, *prefix_lens;
+  void* k;
+  void* v;
+  int32_t* numbers;
+  int64_t batch, total_kv;
+  int32_t window, max_len_extend;
+};
+int launch_unpack_mxfp4(const Mxfp4UnpackArgs& a, hipStream_t stream);
+// mxfp4_norm_rope.hip
+struct Mxfp4NormRopeArgs {
+  Mxfp4Pool pool;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* q_weight;
+  const void* k_weight;
+  const int32_t* positions;
+  const int32_t* out_loc;
+  void* q_out;
+  int64_t q_stride0, k_stride0, v_stride0;  // elements
+  int64_t n_tokens, n_q;
+  double eps, rope_base;
+};
+int launch_norm_rope_store_mxfp4(const Mxfp4NormRopeArgs& a, hipStream_t stream);
+// mxfp4_attention.hip
+struct Mxfp4AttentionArgs {
+  Mxfp4Pool pool;
+  const void* q;
+  const int32_t *kv_indptr, *kv_indices;
+  const int32_t *qo_indptr, *prefix_lens;  // nullptr: decode
+  void* out;
+  void* workspace;
+  int64_t batch, total_kv, n_q;
+  float sm_scale;
+  int32_t max_len_extend, is_cross, window, f16;
+};
+// most columns (queries of a request times q heads of a kv head) of a launch
+int64_t mxfp4_max_columns(int64_t head_dim);
+size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t total_kv, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend);
+int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream);
 
 // A launch without the triple brackets' detour (they put the configuration away and fetch it again, 0.2 us of host time).
 template <typename T>

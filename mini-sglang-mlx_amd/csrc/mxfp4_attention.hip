@@ -1,0 +1,351 @@
+// Attention over a K/V pool in 4 bits (mxfp4.h) for short query blocks: decode, speculative verify, drafts.
+//
+//   out[c] = sum_j w_cj v_j / sum_j w_cj,  w_cj = exp(sm_scale q_c . k_j - m_c),  over the keys j that column c sees
+//
+// Bound by memory: a key of a kv head is D + D / 16 bytes, of its request 4 more, and everything a column needs is computed from one pass
+// over them with the running maximum m and sum.  The visible keys of all requests are one stream, cut into equal segments
+// (splitkv_stream.h); a wave takes a segment for one kv head, and partials of requests that several segments share are merged by a
+// second launch.
+//
+// One wave, 32 keys:
+//   S^T = K Q^T    mfma 16x16x32, keys on M.  Lane (r, g) of the operand holds 32 dims of its key, block 4 h + g of half h: 16 bytes of codes and one
+//                  block byte.  Four products take 8 dims of every block each, which is an order of the contraction like any other, and Q is
+//                  read in the same.
+//   O^T += V^T P^T mfma 16x16x32, dims on M.  Lane (r, g) reads dims 8 r .. 8 r + 7 of half h, one word, of each of the 8 keys of group g, and turns the 8 x 8 values
+//                  over after the conversion.  Row 4 a + i of the two products of S^T is key 8 a + i and 8 a + 4 + i, so the
+//                  weights of group g's keys are the ones that its lanes hold.
+// The conversion multiplies by the block's factor on the way (one instruction for two values), so codes cost what 16-bit values would.
+// Weights are rounded to the type of q for the second product (half a step, 2^-8 and 2^-11 of a weight, as the 16-bit pool's
+// kernels do); scores, sums and accumulators have 32 bits, and so do the partials.
+#include "mxfp4.h"
+#include "splitkv_stream.h"
+
+namespace msgl {
+namespace {
+
+template <int D, int NCT>
+struct MxColumns {
+  u32x4_t q[NCT][D / 32];      // [4 h + c]: dims 128 h + 32 g + 8 c ..
+  int lo[NCT], hi[NCT];        // first and last visible key of this lane's column in each tile of 16
+  int all_lo, all_hi;          // keys inside are visible to every column
+  float m[NCT], l[NCT];        // running maximum (base 2); this lane's part of the sum
+  f32x4_t o[NCT][D / 128][8];  // [h][n][i]: dim 128 h + 8 (4 g + i) + n
+};
+
+template <int D>
+struct MxTile {  // 32 keys as they lie in the pool
+  u32x4_t k[D / 128][2];
+  uint32_t k_byte[D / 128][2];
+  uint32_t v[D / 128][8], v_byte[D / 128][8];
+};
+
+// The factor of a block as the conversion wants it.  Half reaches 65504 = 2^16 (1 - 2^-11) while a block that holds that much has the unit 2^14 and codes up to
+// 6: K and V come in at half their size there, and scores and results are doubled.
+template <bool F16, bool IS_K>
+__device__ __forceinline__ float block_factor(uint32_t byte) {
+  if constexpr (!F16) return mx_scale(byte);
+  else if constexpr (IS_K) return mx_scale(byte == kMxNotFinite ? byte : byte - 1);
+  else return mx_scale(byte - 1);
+}
+template <bool F16>
+constexpr float kBack = F16 ? 2.f : 1.f;
+
+template <int D, int NCT, bool F16>
+__device__ __forceinline__ void start_mx_columns(const SplitKvParams& p, const ReqInfo& r, int kvh, int t_end, MxColumns<D, NCT>& c_) {
+  const int t16 = lane_id() & 15, g = lane_id() >> 4;
+  const int ncols = r.q_len * p.group;
+  int all_lo = 0, all_hi = 0x7fffffff;
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const int col = ct * 16 + t16;
+    const bool valid = col < ncols;
+    const int qi = valid ? query_of(p, col) : 0;
+    const int hh = valid ? col - qi * p.group : 0;
+    const uint16_t* qrow = p.q + (int64_t)(r.q_start + qi) * p.q_stride0 + (kvh * p.group + hh) * D + g * 32;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      c_.q[ct][s] = u32x4_t{0u, 0u, 0u, 0u};
+      if (valid) c_.q[ct][s] = ld_global_b128(qrow + (s >> 2) * 128 + (s & 3) * 8);
+    }
+    const int qpos = r.prefix + qi;
+    int lo = (p.window > 0) ? qpos - p.window + 1 : 0;
+    int hi = min(p.is_cross ? r.kv_len - 1 : min(qpos, r.kv_len - 1), t_end - 1);
+    if (valid) {
+      all_lo = max(all_lo, lo);
+      all_hi = min(all_hi, hi);
+    } else {
+      lo = 1;
+      hi = 0;
+    }
+    c_.lo[ct] = lo;
+    c_.hi[ct] = hi;
+  }
+  c_.all_lo = __builtin_amdgcn_readfirstlane(row_max16(all_lo));
+  c_.all_hi = __builtin_amdgcn_readfirstlane(~row_max16(~all_hi));
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    c_.m[ct] = kNegInf;
+    c_.l[ct] = 0.f;
+#pragma unroll
+    for (int h = 0; h < D / 128; ++h)
+#pragma unroll
+      for (int n = 0; n < 8; ++n) c_.o[ct][h][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// Keys tb .. tb + 31 for the columns in `c_`
+template <int D, int NCT, bool F16>
+__device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const MxTile<D>& t, int tb, MxColumns<D, NCT>& c_) {
+  const int g = lane_id() >> 4;
+  f32x4_t s[2][NCT];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) s[u][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int h = 0; h < D / 128; ++h) {
+      const float factor = block_factor<F16, true>(t.k_byte[h][u]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const u32x4_t k = mx_values8<F16>(t.k[h][u][c], factor);
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) s[u][ct] = mfma_16x16x32_raw<F16>(k, c_.q[ct][4 * h + c], s[u][ct]);
+      }
+    }
+  const bool need_mask = (tb < c_.all_lo) || (tb + 31 > c_.all_hi);
+  u32x4_t pb[NCT];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    float x[8];  // of key tb + 8 g + n
+#pragma unroll
+    for (int n = 0; n < 8; ++n) x[n] = s[n >> 2][ct][n & 3] * p.scale_log2e;
+    if (need_mask) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int key = tb + 8 * g + n;
+        if (key < c_.lo[ct] || key > c_.hi[ct]) x[n] = kNegInf;
+      }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    mx = max_across<32>(max_across<16>(mx));
+    const float m_new = fmaxf(c_.m[ct], mx);
+    const float m_safe = (m_new == kNegInf) ? 0.f : m_new;
+    const float alpha = fast_exp2(c_.m[ct] - m_safe);
+    c_.m[ct] = m_new;
+    float psum = 0.f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      x[n] = fast_exp2(x[n] - m_safe);
+      psum += x[n];
+    }
+    c_.l[ct] = c_.l[ct] * alpha + psum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pb[ct][i] = pack_16x2<F16>(x[2 * i], x[2 * i + 1]);
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+      for (int h = 0; h < D / 128; ++h)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) c_.o[ct][h][n] *= alpha;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < D / 128; ++h) {
+    u32x4_t v[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) v[n] = mx_values8<F16>(t.v[h][n], block_factor<F16, false>(t.v_byte[h][n]));
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      u32x4_t vt;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = v[2 * i][n >> 1], b = v[2 * i + 1][n >> 1];
+        vt[i] = (n & 1) ? pack_hi16(a, b) : pack_lo16(a, b);
+      }
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) c_.o[ct][h][n] = mfma_16x16x32_raw<F16>(vt, pb[ct], c_.o[ct][h][n]);
+    }
+  }
+}
+
+// Keys [t_begin, t_end) of request `r`, in order, for the columns in `c_`
+template <int D, int NCT, bool F16>
+__device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const ReqInfo& r, int kvh, int t_begin, int t_end, MxColumns<D, NCT>& c_) {
+  const int t16 = lane_id() & 15, g = lane_id() >> 4;
+  const unsigned char* codes = reinterpret_cast<const unsigned char*>(p.k_cache) + kvh * D;
+  const unsigned char* scales = reinterpret_cast<const unsigned char*>(p.v_cache) + kvh * (D / 16);
+  const int32_t* idx = p.kv_indices + r.kv_start;
+  auto slot_of = [&](int key) { return (int64_t)min((uint32_t)idx[min(key, t_end - 1)], p.max_slot); };
+  for (int tb = t_begin; tb < t_end; tb += 32) {
+    MxTile<D> t;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t slot = slot_of(tb + 8 * (t16 >> 2) + 4 * u + (t16 & 3));
+#pragma unroll
+      for (int h = 0; h < D / 128; ++h) {
+        t.k[h][u] = ld_global_b128(codes + slot * p.k_stride0 + (4 * h + g) * 16);
+        t.k_byte[h][u] = scales[slot * p.v_stride0 + 4 * h + g];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int64_t slot = slot_of(tb + 8 * g + n);
+#pragma unroll
+      for (int h = 0; h < D / 128; ++h) {
+        t.v[h][n] = *reinterpret_cast<const uint32_t*>(codes + slot * p.k_stride0 + D / 2 + h * 64 + t16 * 4);
+        t.v_byte[h][n] = scales[slot * p.v_stride0 + D / 32 + 4 * h + (t16 >> 2)];
+      }
+    }
+    compute_mx_tile<D, NCT, F16>(p, t, tb, c_);
+  }
+}
+
+// A request's share is done: its rows, if the segment held all of it, else its partial.
+template <int D, int NCT, bool F16>
+__device__ __forceinline__ void leave_share(const SplitKvParams& p, const ReqInfo& r, int seg, int b, int kvh, bool whole, MxColumns<D, NCT>& c_) {
+  const int t16 = lane_id() & 15, g = lane_id() >> 4;
+  const int ncols = r.q_len * p.group;
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const float l = sum_across<32>(sum_across<16>(c_.l[ct]));
+    const float inv = (l > 0.f) ? kBack<F16> / l : 0.f;  // (NaN: the accumulators are that too)
+    const int col = ct * 16 + t16;
+    if (col >= ncols) continue;
+    if (whole) {
+      const int qi = query_of(p, col), hh = col - qi * p.group;
+      uint16_t* orow = p.out + ((int64_t)(r.q_start + qi) * p.n_q + kvh * p.group + hh) * D;
+#pragma unroll
+      for (int h = 0; h < D / 128; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u32x4_t w;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) w[n] = pack_16x2<F16>(c_.o[ct][h][2 * n][i] * inv, c_.o[ct][h][2 * n + 1][i] * inv);
+          st_global_b128(orow + h * 128 + (4 * g + i) * 8, w);
+        }
+    } else {
+      const int64_t block = (int64_t)(seg + b) * p.n_kv + kvh;
+#pragma unroll
+      for (int h = 0; h < D / 128; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4_t w0, w1;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            w0[n] = c_.o[ct][h][n][i] * inv;
+            w1[n] = c_.o[ct][h][4 + n][i] * inv;
+          }
+          float* dst = p.part_o + partial_offset(block, p.cols, col, h * 128 + (4 * g + i) * 8, D);
+          *reinterpret_cast<f32x4_t*>(dst) = w0;
+          *reinterpret_cast<f32x4_t*>(dst + 4) = w1;
+        }
+      // NaN: any weight above zero takes the partial's NaN into the merged row
+      if (g == 0) p.part_lse[block * p.cols + col] = l > 0.f ? c_.m[ct] + __log2f(l) : l == 0.f ? kNegInf : 0.f;
+    }
+  }
+}
+
+template <int D, int NCT, bool F16>
+__global__ __launch_bounds__(256) void mxfp4_attention_kernel(SplitKvParams p) {
+  const int seg = blockIdx.x / p.head_groups;
+  const int kvh = (blockIdx.x - seg * p.head_groups) * p.nwh + (threadIdx.x >> 6);
+  int seg_len, total, b, vs;
+  if (!locate_segment(p, seg, &seg_len, &total, &b, &vs)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  vs = __builtin_amdgcn_readfirstlane(vs);
+  int vpos = seg * seg_len;
+  const int seg_end = min(vpos + seg_len, total);
+  while (vpos < seg_end && b < p.batch) {
+    const ReqInfo r = request_info(p, b);
+    const int vlen = r.hi - r.lo;
+    if (vpos >= vs + vlen) {  // no keys, or past them in the empty positions: on to the next request
+      vs += stream_length(p, vlen);
+      vpos = max(vpos, vs);
+      ++b;
+      continue;
+    }
+    const int t_begin = r.lo + (vpos - vs);
+    const int t_end = min(r.hi, t_begin + (seg_end - vpos));
+    if (t_begin == r.lo && kvh == 0 && lane_id() == 0) {
+      // the wave that starts a request tells the merge kernel where its partials are
+      const int s_first = vs / seg_len;
+      p.req_items[2 * b] = s_first;
+      p.req_items[2 * b + 1] = (vs + vlen - 1) / seg_len - s_first + 1;
+    }
+    MxColumns<D, NCT> c_;
+    start_mx_columns<D, NCT, F16>(p, r, kvh, t_end, c_);
+    attend_mx_keys<D, NCT, F16>(p, r, kvh, t_begin, t_end, c_);
+    leave_share<D, NCT, F16>(p, r, seg, b, kvh, t_begin == r.lo && t_end == r.hi, c_);
+    vpos += t_end - t_begin;
+  }
+}
+
+constexpr int kMinSegment = 64;
+int heads_per_group(int64_t n_kv) { return n_kv % 4 == 0 ? 4 : n_kv % 2 == 0 ? 2 : 1; }
+int segments(int64_t total_kv, int64_t n_kv) {
+  const int64_t waves = (int64_t)device_cus() * 8;
+  return (int)std::max<int64_t>(1, std::min(waves / n_kv, (total_kv + kMinSegment - 1) / kMinSegment));
+}
+
+}  // namespace
+
+int64_t mxfp4_max_columns(int64_t head_dim) { return head_dim == 128 ? 64 : 32; }
+
+size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t total_kv, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend) {
+  return splitkv_workspace_bytes(batch, n_q, n_kv, head_dim, max_len_extend, segments(total_kv, n_kv));
+}
+
+int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
+  const int64_t n_kv = a.pool.n_kv, d = a.pool.head_dim, cols = a.n_q / n_kv * a.max_len_extend;
+  if (cols < 1 || cols > mxfp4_max_columns(d)) return MSGL_ERR_SHAPE;
+  SplitKvParams p{};
+  p.q = static_cast<const uint16_t*>(a.q);
+  p.k_cache = static_cast<const uint16_t*>(a.pool.codes);   // as bytes, strides too
+  p.v_cache = static_cast<const uint16_t*>(a.pool.scales);
+  p.k_stride0 = a.pool.codes_stride0;
+  p.v_stride0 = a.pool.scales_stride0;
+  p.kv_indptr = a.kv_indptr;
+  p.kv_indices = a.kv_indices;
+  p.qo_indptr = a.qo_indptr;
+  p.prefix_lens = a.prefix_lens;
+  p.out = static_cast<uint16_t*>(a.out);
+  p.q_stride0 = a.n_q * d;
+  p.batch = (int32_t)a.batch;
+  p.n_q = (int32_t)a.n_q;
+  p.n_kv = (int32_t)n_kv;
+  p.group = (int32_t)(a.n_q / n_kv);
+  p.per_group = 65535u / (uint32_t)p.group + 1u;
+  p.cols = (int32_t)cols;
+  p.nwh = heads_per_group(n_kv);
+  p.head_groups = (int32_t)(n_kv / p.nwh);
+  p.n_seg = segments(a.total_kv, n_kv);
+  p.min_seg = kMinSegment;
+  p.max_len_extend = p.q_cap = a.max_len_extend;
+  p.f16 = a.f16;
+  p.is_cross = a.is_cross;
+  p.window = a.window;
+  p.max_slot = (uint32_t)(a.pool.num_slots - 1);
+  p.scale_log2e = a.sm_scale * kLog2e * (a.f16 ? 2.f : 1.f);
+  const int64_t rows = ((int64_t)p.n_seg + a.batch) * n_kv * cols;
+  char* ws = static_cast<char*>(a.workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_lse = reinterpret_cast<float*>(ws + (size_t)rows * d * sizeof(float));
+  p.req_items = reinterpret_cast<int32_t*>(ws + (size_t)rows * (d + 1) * sizeof(float));
+  auto launch = [&](auto kernel) {
+    return launch_kernel(kernel, dim3((unsigned)(p.n_seg * p.head_groups)), dim3(64 * p.nwh), stream, p);
+  };
+  const int nct = (int)((cols + 15) / 16);
+  int rc;
+  if (a.f16 && nct > 1) return MSGL_ERR_DTYPE;
+  if (d == 128)
+    rc = launch(a.f16      ? mxfp4_attention_kernel<128, 1, true>
+                : nct == 1 ? mxfp4_attention_kernel<128, 1, false>
+                : nct == 2 ? mxfp4_attention_kernel<128, 2, false>
+                           : mxfp4_attention_kernel<128, 4, false>);
+  else
+    rc = launch(a.f16 ? mxfp4_attention_kernel<256, 1, true> : nct == 1 ? mxfp4_attention_kernel<256, 1, false> : mxfp4_attention_kernel<256, 2, false>);
+  return rc != MSGL_OK ? rc : launch_fp32_merge(p, d, stream);
+}
+
+}  // namespace msgl

@@ -1,5 +1,5 @@
 // The Python call path of the operators: argument checks, output and workspace allocation and the
-// call into the C ABI (include/msgl_paged_attention.h), as one CPython extension module
+// call into the C ABI (include/msgl_paged_attention.h, include/msgl_mxfp4_cache.h), as one CPython extension module
 // (mini_sglang_amd_kernel/_native.so).  Host code only, compiled by g++ against torch's headers.
 //
 // Why it is native: at serving's small sizes a layer's kernels take 10-30 us, and the same steps
@@ -31,6 +31,7 @@
 #include <utility>
 #include <vector>
 
+#include "../../include/msgl_mxfp4_cache.h"
 #include "../../include/msgl_paged_attention.h"
 
 namespace {
@@ -766,6 +767,229 @@ PyObject* gdn_state_inplace(PyObject*, PyObject* const* args, Py_ssize_t n_args)
   });
 }
 
+// ---- the pool in 4 bits (include/msgl_mxfp4_cache.h) ------------------------------------------------
+Wrong mxfp4_pool(const Tensor& codes, const Tensor& scales, int64_t n_kv, int64_t d) {
+  if (codes.dim() != 4 || scales.dim() != 4 || codes.size(2) != 2 || scales.size(2) != 2)
+    return "kv_codes and kv_scales must be 4D (num_pages, num_kv_heads, 2, head_dim / 2) and (num_pages, num_kv_heads, 2, head_dim / 32)";
+  if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte) return "kv_codes and kv_scales must be uint8";
+  if (d != 128 && d != 256) return "head_dim must be 128 or 256";
+  if (codes.size(1) != n_kv || scales.size(1) != n_kv || codes.size(3) * 2 != d || scales.size(3) * 32 != d)
+    return "kv_codes and kv_scales must be (num_pages, num_kv_heads, 2, head_dim / 2) and (num_pages, num_kv_heads, 2, head_dim / 32)";
+  if (codes.size(0) != scales.size(0)) return "kv_codes and kv_scales must have as many pages";
+  if (codes.size(0) == 0) return "kv_codes and kv_scales must have a page";
+  for (const Tensor* t : {&codes, &scales})
+    if (t->stride(3) != 1 || t->stride(2) != t->size(3) || t->stride(1) != 2 * t->size(3))
+      return "kv_codes and kv_scales must be contiguous behind their first dimension";
+  return {};
+}
+int64_t page_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2) * t.size(3); }
+
+Wrong type16(const Tensor& t, const char* name) {
+  return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf ? Wrong() : Wrong(name, " must be float16 or bfloat16");
+}
+// Rows as the kernels read them: 16 bytes at a time, heads one behind the other
+bool aligned_rows(const Tensor& t) {
+  return whole_rows(t) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_stride(t) % 8 == 0 && row_stride(t) >= t.size(1) * t.size(2);
+}
+Tensor rows_of(const Tensor& t) { return aligned_rows(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+Tensor aligned(const Tensor& t) {  // contiguous, at 16 bytes
+  return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// store_kv_cache_mxfp4(kv_codes, kv_scales, indices, k, v, validate)
+PyObject* store_kv_cache_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded(args, n_args, 6, [](PyObject* const* a) -> PyObject* {
+    static const char op[] = "store_kv_cache_mxfp4";
+    const Tensor &codes = tensor(a[0], "kv_codes"), &scales = tensor(a[1], "kv_scales"), &idx = tensor(a[2], "indices");
+    const Tensor &k = tensor(a[3], "k"), &v = tensor(a[4], "v");
+    if (idx.dim() != 1) fail(op, "indices must be 1D");
+    if (k.dim() != 3 || v.dim() != 3) fail(op, "k and v must be 3D (length, num_kv_heads, head_dim)");
+    require(op, type16(k, "k"));
+    if (v.scalar_type() != k.scalar_type()) fail(op, "k and v must have the same dtype");
+    require_int32(op, idx, "indices");
+    if (k.size(0) != idx.size(0) || v.sizes() != k.sizes()) fail(op, "k and v shape must be (length, num_kv_heads, head_dim)");
+    require(op, mxfp4_pool(codes, scales, k.size(1), k.size(2)));
+    const c10::Device dev = require_device(op, {&codes, &scales, &idx, &k, &v});
+    const int64_t length = idx.size(0);
+    if (length == 0) return none();
+    debug_checks(a[5], op, {a[2], a[0]});
+    int rc;
+    {
+      NoGil nogil;
+      OnDevice on(dev);
+      const Tensor ks = rows_of(k), vs = rows_of(v), ix = idx.contiguous();
+      rc = msgl_store_kv_cache_mxfp4(codes.data_ptr(), scales.data_ptr(), ints(ix), ks.data_ptr(), vs.data_ptr(), length, k.size(1), k.size(2),
+                                     codes.size(0), page_stride(codes), page_stride(scales), row_stride(ks), row_stride(vs), dtype_code(k), on.ptr());
+    }
+    check_rc(op, rc);
+    return none();
+  });
+}
+
+// load_kv_cache_mxfp4(kv_codes, kv_scales, indices, half, validate) -> (k, v)
+PyObject* load_kv_cache_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded(args, n_args, 5, [](PyObject* const* a) -> PyObject* {
+    static const char op[] = "load_kv_cache_mxfp4";
+    const Tensor &codes = tensor(a[0], "kv_codes"), &scales = tensor(a[1], "kv_scales"), &idx = tensor(a[2], "indices");
+    const bool half = truth(a[3]);
+    if (idx.dim() != 1) fail(op, "indices must be 1D");
+    require_int32(op, idx, "indices");
+    if (codes.dim() != 4) fail(op, "kv_codes must be 4D (num_pages, num_kv_heads, 2, head_dim / 2)");
+    const int64_t n_kv = codes.size(1), d = 2 * codes.size(3), length = idx.size(0);
+    require(op, mxfp4_pool(codes, scales, n_kv, d));
+    const c10::Device dev = require_device(op, {&codes, &scales, &idx});
+    if (length > 0) debug_checks(a[4], op, {a[2], a[0]});
+    Tensor k, v;
+    int rc;
+    {
+      NoGil nogil;
+      OnDevice on(dev);
+      const Tensor both = empty({2, length, n_kv, d}, half ? at::kHalf : at::kBFloat16, dev), ix = idx.contiguous();
+      k = both.select(0, 0);
+      v = both.select(0, 1);
+      rc = msgl_load_kv_cache_mxfp4(codes.data_ptr(), scales.data_ptr(), ints(ix), k.data_ptr(), v.data_ptr(), length, n_kv, d, codes.size(0),
+                                    page_stride(codes), page_stride(scales), half ? MSGL_DTYPE_F16 : MSGL_DTYPE_BF16, on.ptr());
+    }
+    check_rc(op, rc);
+    PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
+    PyObject* pair = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
+    Py_XDECREF(pk);
+    Py_XDECREF(pv);
+    if (!pair) throw PyFailure();
+    return pair;
+  });
+}
+
+// qk_norm_rope_store_mxfp4(q, k, v, q_weight, k_weight, positions, out_loc, kv_codes, kv_scales, eps, rope_base, validate) -> q
+PyObject* qk_norm_rope_store_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded(args, n_args, 12, [](PyObject* const* a) -> PyObject* {
+    static const char op[] = "qk_norm_rope_store_mxfp4";
+    const Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &qw = tensor(a[3], "q_weight");
+    const Tensor &kw = tensor(a[4], "k_weight"), &pos = tensor(a[5], "positions"), &loc = tensor(a[6], "out_loc");
+    const Tensor &codes = tensor(a[7], "kv_codes"), &scales = tensor(a[8], "kv_scales");
+    const std::pair<const Tensor*, const char*> typed[] = {{&q, "q"}, {&k, "k"}, {&v, "v"}, {&qw, "q_weight"}, {&kw, "k_weight"}};
+    for (int i = 0; i < 3; ++i)
+      if (typed[i].first->dim() != 3) fail(op, std::string(typed[i].second) + " must be 3D (tokens, heads, head_dim)");
+    for (const auto& [t, name] : typed)
+      if (t->scalar_type() != at::kBFloat16) fail(op, std::string(name) + " must be bfloat16");
+    const int64_t tokens = q.size(0), n_q = q.size(1), d = q.size(2), n_kv = k.size(1);
+    if (n_q == 0) fail(op, "q must have a head");
+    require(op, mxfp4_pool(codes, scales, n_kv, d));
+    if (k.size(0) != tokens || k.size(2) != d || v.sizes() != k.sizes()) fail(op, "k and v shape must be (tokens, num_kv_heads, head_dim)");
+    if (qw.dim() != 1 || qw.size(0) != d || kw.dim() != 1 || kw.size(0) != d) fail(op, "q_weight and k_weight must be (head_dim,)");
+    require_int32(op, pos, "positions");
+    require_int32(op, loc, "out_loc");
+    if (pos.dim() != 1 || loc.dim() != 1 || pos.size(0) != tokens || loc.size(0) != tokens)
+      fail(op, "positions and out_loc length must match q length");
+    const c10::Device dev = require_device(op, {&q, &k, &v, &qw, &kw, &pos, &loc, &codes, &scales});
+    const double eps = real(a[9]), base = real(a[10]);
+    if (tokens > 0) debug_checks(a[11], op, {a[6], a[7]});
+    Tensor out;
+    int rc;
+    {
+      NoGil nogil;
+      OnDevice on(dev);
+      out = empty({tokens, n_q, d}, at::kBFloat16, dev);
+      const Tensor qs = rows_of(q), ks = rows_of(k), vs = rows_of(v), qwc = aligned(qw), kwc = aligned(kw), pc = pos.contiguous(), lc = loc.contiguous();
+      rc = msgl_qk_norm_rope_store_mxfp4(qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), row_stride(qs), row_stride(ks), row_stride(vs), qwc.data_ptr(),
+                                         kwc.data_ptr(), ints(pc), ints(lc), out.data_ptr(), codes.data_ptr(), scales.data_ptr(), page_stride(codes),
+                                         page_stride(scales), codes.size(0), tokens, n_q, n_kv, d, eps, base, MSGL_DTYPE_BF16, on.ptr());
+    }
+    check_rc(op, rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// paged_decode_attention_mxfp4(q, kv_codes, kv_scales, kv_indptr, kv_indices, sm_scale, validate) -> out
+PyObject* paged_decode_attention_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded(args, n_args, 7, [](PyObject* const* a) -> PyObject* {
+    static const char op[] = "paged_decode_attention_mxfp4";
+    const Tensor &q = tensor(a[0], "q"), &codes = tensor(a[1], "kv_codes"), &scales = tensor(a[2], "kv_scales");
+    const Tensor &ip = tensor(a[3], "kv_indptr"), &ix = tensor(a[4], "kv_indices");
+    if (q.dim() != 3) fail(op, "q must be 3D (batch, num_q_heads, head_dim)");
+    if (ip.dim() != 1 || ix.dim() != 1) fail(op, "kv_indptr and kv_indices must be 1D");
+    if (codes.dim() != 4) fail(op, "kv_codes must be 4D (num_pages, num_kv_heads, 2, head_dim / 2)");
+    const int64_t batch = q.size(0), n_q = q.size(1), d = q.size(2), n_kv = codes.size(1), total_kv = ix.size(0);
+    if (n_q == 0 || n_kv == 0 || n_q % n_kv != 0) fail(op, "num_q_heads must be a multiple of num_kv_heads");
+    if (n_q / n_kv > 16) fail(op, "only q_heads/kv_heads <= 16 is supported");
+    require(op, mxfp4_pool(codes, scales, n_kv, d));
+    require(op, type16(q, "q"));
+    require_int32(op, ip, "kv_indptr");
+    require_int32(op, ix, "kv_indices");
+    if (ip.size(0) != batch + 1) fail(op, "kv_indptr must have batch + 1 entries");
+    const c10::Device dev = require_device(op, {&q, &codes, &scales, &ip, &ix});
+    const float scale = static_cast<float>(real(a[5]));
+    if (batch > 0) debug_checks(a[6], op, {a[3], a[4], a[1]});
+    Tensor out;
+    int rc = MSGL_OK;
+    {
+      NoGil nogil;
+      OnDevice on(dev);
+      out = empty({batch, n_q, d}, q.scalar_type(), dev);
+      if (batch > 0) {
+        const Tensor qc = aligned(q), ipc = ip.contiguous(), ixc = ix.contiguous();
+        const size_t bytes = msgl_paged_decode_mxfp4_workspace_bytes(batch, total_kv, n_q, n_kv, d);
+        const Scratch ws(bytes, on);
+        rc = msgl_paged_decode_attention_mxfp4(qc.data_ptr(), codes.data_ptr(), scales.data_ptr(), ints(ipc), ints(ixc), out.data_ptr(), ws.ptr(), bytes,
+                                               batch, total_kv, n_q, n_kv, d, codes.size(0), page_stride(codes), page_stride(scales), scale,
+                                               dtype_code(q), on.ptr());
+      }
+    }
+    check_rc(op, rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// paged_prefill_attention_mxfp4(q, kv_codes, kv_scales, qo_indptr, kv_indptr, kv_indices, prefix_lens, sm_scale, max_len_extend,
+//                               is_cross_attention, sliding_window_size, validate) -> out
+PyObject* paged_prefill_attention_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded(args, n_args, 12, [](PyObject* const* a) -> PyObject* {
+    static const char op[] = "paged_prefill_attention_mxfp4";
+    const Tensor &q = tensor(a[0], "q"), &codes = tensor(a[1], "kv_codes"), &scales = tensor(a[2], "kv_scales");
+    const Tensor &qp = tensor(a[3], "qo_indptr"), &ip = tensor(a[4], "kv_indptr"), &ix = tensor(a[5], "kv_indices");
+    const Tensor& pl = tensor(a[6], "prefix_lens");
+    if (q.dim() != 3) fail(op, "q must be 3D (total_q_tokens, num_q_heads, head_dim)");
+    if (qp.dim() != 1 || ip.dim() != 1 || ix.dim() != 1 || pl.dim() != 1) fail(op, "qo_indptr, kv_indptr, kv_indices, prefix_lens must be 1D");
+    if (codes.dim() != 4) fail(op, "kv_codes must be 4D (num_pages, num_kv_heads, 2, head_dim / 2)");
+    const int64_t total_q = q.size(0), n_q = q.size(1), d = q.size(2), n_kv = codes.size(1), batch = qp.size(0) - 1, total_kv = ix.size(0);
+    if (n_q == 0 || n_kv == 0 || n_q % n_kv != 0) fail(op, "num_q_heads must be a multiple of num_kv_heads");
+    require(op, mxfp4_pool(codes, scales, n_kv, d));
+    const int64_t window = integer(a[10]);
+    if (window < 0) fail(op, "sliding_window_size must be >= 0");
+    if (batch <= 0) fail(op, "batch must be > 0");
+    if (q.scalar_type() != at::kBFloat16) fail(op, "unsupported dtype, the prefill kernel is bfloat16 only");
+    require_int32(op, qp, "qo_indptr");
+    require_int32(op, ip, "kv_indptr");
+    require_int32(op, ix, "kv_indices");
+    require_int32(op, pl, "prefix_lens");
+    if (ip.size(0) != batch + 1 || pl.size(0) != batch) fail(op, "kv_indptr / prefix_lens length must match qo_indptr");
+    const float scale = static_cast<float>(real(a[7]));
+    const int64_t max_extend = integer(a[8]);
+    if (max_extend > 0x7fffffff || window > 0x7fffffff) fail(op, "max_len_extend and sliding_window_size must fit 32 bits");
+    const c10::Device dev = require_device(op, {&q, &codes, &scales, &qp, &ip, &ix, &pl});
+    const bool cross = truth(a[9]);
+    if (total_q > 0) debug_checks(a[11], op, {a[3], a[4], a[5], a[0], a[1]});
+    Tensor out;
+    int rc = MSGL_OK;
+    {
+      NoGil nogil;
+      OnDevice on(dev);
+      out = empty({total_q, n_q, d}, q.scalar_type(), dev);
+      if (total_q > 0) {
+        const Tensor qc = aligned(q), qpc = qp.contiguous(), ipc = ip.contiguous(), ixc = ix.contiguous(), plc = pl.contiguous();
+        const size_t bytes = msgl_paged_prefill_mxfp4_workspace_bytes(batch, total_q, total_kv, n_q, n_kv, d, max_extend);
+        const Scratch ws(bytes, on);
+        rc = msgl_paged_prefill_attention_mxfp4(qc.data_ptr(), codes.data_ptr(), scales.data_ptr(), ints(qpc), ints(ipc), ints(ixc), ints(plc),
+                                                out.data_ptr(), ws.ptr(), bytes, batch, total_q, total_kv, n_q, n_kv, d, codes.size(0),
+                                                page_stride(codes), page_stride(scales), scale, static_cast<int32_t>(max_extend), cross ? 1 : 0,
+                                                static_cast<int32_t>(window), MSGL_DTYPE_BF16, on.ptr());
+      }
+    }
+    check_rc(op, rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 PyObject* set_checks(PyObject*, PyObject* fn) {
   Py_INCREF(fn);
   Py_XSETREF(g_run_checks, fn);
@@ -782,6 +1006,11 @@ PyMethodDef g_methods[] = {MSGL_FAST(store_kv_cache),
                            MSGL_FAST(decode_step),
                            MSGL_FAST(extend_step),
                            MSGL_FAST(gdn_state_inplace),
+                           MSGL_FAST(store_kv_cache_mxfp4),
+                           MSGL_FAST(load_kv_cache_mxfp4),
+                           MSGL_FAST(qk_norm_rope_store_mxfp4),
+                           MSGL_FAST(paged_decode_attention_mxfp4),
+                           MSGL_FAST(paged_prefill_attention_mxfp4),
                            {"set_checks", set_checks, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -18,8 +18,10 @@ from typing import List, Optional, Sequence
 import torch
 
 from mini_sglang_amd.kvcache.mha_pool import MHAKVCache
+from mini_sglang_amd.kvcache.mxfp4_pool import MXFP4KVCache
 from mini_sglang_amd_kernel import (_native, build_metadata_from_host, paged_decode_attention,
-                                    paged_prefill_attention, qk_norm_rope_store)
+                                    paged_decode_attention_mxfp4, paged_prefill_attention,
+                                    paged_prefill_attention_mxfp4, qk_norm_rope_store, qk_norm_rope_store_mxfp4)
 
 MAX_KV_SPLITS = 32
 
@@ -67,7 +69,8 @@ AttnMetadata = PrefillMetadata | DecodeMetadata
 class AttnBackend:
     """Paged attention backend for MI355X using the msgl HIP kernels.
 
-    ``config`` needs ``head_dim``; ``kvcache`` is a ``BaseKVCache``; ``page_table`` is the
+    ``config`` needs ``head_dim``; ``kvcache`` is a ``BaseKVCache`` (with an ``MXFP4KVCache`` every step is its store and its
+    attention over codes, whatever ``own_slots`` says); ``page_table`` is the
     ``(max_running_req + 1, max_seq_len)`` int32 slot table the scheduler fills.
     """
 
@@ -115,6 +118,8 @@ class AttnBackend:
         if out is not None:
             return out
         self.kvcache.store_kv(k, v, batch.out_loc, layer_id)
+        if isinstance(cache, MXFP4KVCache):
+            return self._attend_mxfp4(q, layer_id, metadata, is_cross_attention, sliding_window_size)
         k_cache = self.kvcache.k_cache(layer_id)
         v_cache = self.kvcache.v_cache(layer_id)
         return self._attend(q, k_cache, v_cache, metadata, is_cross_attention, sliding_window_size)
@@ -135,6 +140,20 @@ class AttnBackend:
         return paged_decode_attention(
             q, k_cache, v_cache, metadata.kv_indptr, metadata.kv_indices, metadata.num_kv_splits,
             sm_scale=self.sm_scale, max_kv_splits=metadata.max_kv_splits)
+
+    def _attend_mxfp4(self, q, layer_id: int, metadata, is_cross_attention: bool, sliding_window_size: int) -> torch.Tensor:
+        codes, scales = self.kvcache.codes(layer_id), self.kvcache.scales(layer_id)
+        if isinstance(metadata, PrefillMetadata):
+            return paged_prefill_attention_mxfp4(
+                q, codes, scales, metadata.qo_indptr, metadata.kv_indptr, metadata.kv_indices, metadata.prefix_lens,
+                sm_scale=self.sm_scale, max_len_extend=metadata.max_len_extend,
+                is_cross_attention=is_cross_attention, sliding_window_size=sliding_window_size)
+        assert isinstance(metadata, DecodeMetadata)
+        assert not is_cross_attention and sliding_window_size == 0, (
+            "is_cross_attention / sliding_window_size are only "
+            "supported on the prefill path."
+        )
+        return paged_decode_attention_mxfp4(q, codes, scales, metadata.kv_indptr, metadata.kv_indices, sm_scale=self.sm_scale)
 
     def forward_fused_norm_rope(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                 q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor,
@@ -160,6 +179,10 @@ class AttnBackend:
                                       rms_norm_eps, rope_base)
             if out is not None:
                 return out
+        if isinstance(cache, MXFP4KVCache):
+            q = qk_norm_rope_store_mxfp4(q, k, v, q_norm_weight, k_norm_weight, metadata.positions, batch.out_loc,
+                                         cache.codes(layer_id), cache.scales(layer_id), eps=rms_norm_eps, rope_base=rope_base)
+            return self._attend_mxfp4(q, layer_id, metadata, is_cross_attention, sliding_window_size)
         k_cache = self.kvcache.k_cache(layer_id)
         v_cache = self.kvcache.v_cache(layer_id)
         q = qk_norm_rope_store(q, k, v, q_norm_weight, k_norm_weight, metadata.positions,

@@ -9,6 +9,7 @@ import torch
 from .base import BaseCacheHandle, BaseCacheManager, BaseKVCache, SizeInfo
 from .mamba_pool import MambaStateConfig, MambaStatePool, MambaStateShape
 from .mha_pool import MHAKVCache
+from .mxfp4_pool import MXFP4KVCache
 from .radix_manager import (HybridCacheHandle, HybridRadixCacheManager, RadixCacheHandle,
                             RadixCacheManager, RadixTreeNode)
 
@@ -51,10 +52,16 @@ class NaiveCacheManager(BaseCacheManager):
         return None
 
 
-def create_kvcache(model_config, num_pages: int, dtype: torch.dtype, device="cuda") -> BaseKVCache:
-    """K/V pools for a model described by ``num_kv_heads`` / ``num_layers`` / ``head_dim``."""
-    return MHAKVCache(num_kv_heads=model_config.num_kv_heads, num_layers=model_config.num_layers,
-                      head_dim=model_config.head_dim, num_pages=num_pages, dtype=dtype, device=device)
+SUPPORTED_KV_FORMAT: Dict[str, Callable[..., BaseKVCache]] = {"16bit": MHAKVCache, "mxfp4": MXFP4KVCache}
+
+
+def create_kvcache(model_config, num_pages: int, dtype: torch.dtype, device="cuda", kv_format: str = "16bit") -> BaseKVCache:
+    """K/V pools for a model described by ``num_kv_heads`` / ``num_layers`` / ``head_dim``; ``kv_format``
+    "mxfp4": 4-bit floats under a power of two to 32 of them (the reference's pools are 16 bits)."""
+    if kv_format not in SUPPORTED_KV_FORMAT:
+        raise KeyError(f"Unsupported KV format: {kv_format!r}; known: {sorted(SUPPORTED_KV_FORMAT)}")
+    return SUPPORTED_KV_FORMAT[kv_format](num_kv_heads=model_config.num_kv_heads, num_layers=model_config.num_layers,
+                                          head_dim=model_config.head_dim, num_pages=num_pages, dtype=dtype, device=device)
 
 
 SUPPORTED_CACHE_MANAGER: Dict[str, Callable[..., BaseCacheManager]] = {
@@ -73,8 +80,8 @@ def create_hybrid_radix_cache_manager(mamba_pool: MambaStatePool, device=None) -
     return HybridRadixCacheManager(mamba_pool=mamba_pool, device=device)
 
 
-__all__ = ["BaseKVCache", "MHAKVCache", "BaseCacheHandle", "BaseCacheManager", "SizeInfo",
+__all__ = ["BaseKVCache", "MHAKVCache", "MXFP4KVCache", "BaseCacheHandle", "BaseCacheManager", "SizeInfo",
            "RadixTreeNode", "RadixCacheHandle", "RadixCacheManager", "HybridCacheHandle",
            "HybridRadixCacheManager", "NaiveCacheHandle", "NaiveCacheManager", "MambaStateShape",
            "MambaStateConfig", "MambaStatePool", "create_kvcache", "create_cache_manager",
-           "create_hybrid_radix_cache_manager", "SUPPORTED_CACHE_MANAGER"]
+           "create_hybrid_radix_cache_manager", "SUPPORTED_CACHE_MANAGER", "SUPPORTED_KV_FORMAT"]

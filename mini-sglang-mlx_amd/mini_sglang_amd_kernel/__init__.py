@@ -30,7 +30,9 @@ except ImportError as _exc:  # not built: the first call says so
 __all__ = ["store_kv_cache", "paged_decode_attention", "paged_prefill_attention",
            "build_attention_metadata", "build_metadata_from_host", "qk_norm_rope_store", "decode_step", "extend_step",
            "gdn_state_inplace",
-           "fast_compare_key"]
+           "fast_compare_key",
+           "store_kv_cache_mxfp4", "load_kv_cache_mxfp4", "qk_norm_rope_store_mxfp4", "paged_decode_attention_mxfp4",
+           "paged_prefill_attention_mxfp4"]
 
 
 def _fail(op: str, msg: str):
@@ -118,13 +120,16 @@ def _run_checks(validate, op: str, *args) -> None:
     arrays and the tensors they point into."""
     if not _checks_on(validate):
         return
-    if op == "store_kv_cache":
+    if op in ("store_kv_cache", "store_kv_cache_mxfp4"):
         indices, k_cache = args
         _validate_slot_ids(op, "indices", indices, k_cache.shape[0], unique=True)
-    elif op == "qk_norm_rope_store":
+    elif op == "load_kv_cache_mxfp4":
+        indices, k_cache = args
+        _validate_slot_ids(op, "indices", indices, k_cache.shape[0])
+    elif op in ("qk_norm_rope_store", "qk_norm_rope_store_mxfp4"):
         out_loc, k_cache = args
         _validate_slot_ids(op, "out_loc", out_loc, k_cache.shape[0], unique=True)
-    elif op == "paged_decode_attention":
+    elif op in ("paged_decode_attention", "paged_decode_attention_mxfp4"):
         kv_indptr, kv_indices, k_cache = args
         _validate_indptr(op, "kv_indptr", kv_indptr, kv_indices.shape[0], "kv_indices")
         _validate_slot_ids(op, "kv_indices", kv_indices, k_cache.shape[0])
@@ -318,6 +323,85 @@ def gdn_state_inplace(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     with _on_stream(stream, q):
         return _native.gdn_state_inplace(q, k, v, g, beta, state, slot_ids, qo_indptr,
                                          single_token_mode, max_len_extend)
+
+
+# ---- the pool in 4 bits ------------------------------------------------------------------------
+# ``kv_codes`` is ``(num_pages, num_kv_heads, 2, head_dim // 2)`` and ``kv_scales`` ``(num_pages, num_kv_heads, 2,
+# head_dim // 32)``, uint8, K first: 4-bit floats (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign; dim 2i in the low half of byte
+# i) times ``2 ** (b - 127)`` of the block of 32 dims they belong to.  ``mini_sglang_amd.kvcache.MXFP4KVCache`` holds both for all layers.
+def store_kv_cache_mxfp4(kv_codes: torch.Tensor, kv_scales: torch.Tensor, indices: torch.Tensor,
+                         k: torch.Tensor, v: torch.Tensor, *, stream=None,
+                         validate: Optional[bool] = None) -> None:
+    """``store_kv_cache`` into a pool of 4 bits: rows ``k[r]`` and ``v[r]`` (bf16 or float16) as codes at slot ``indices[r]``.
+
+    A block's factor is the smallest power of two with which none of its values lies beyond 6, from 2^-125 to 2^125; values go to the
+    nearest code, halfway to the even one.  A head whose row of k or v is not finite is stored as a key that gives NaN to every query
+    that sees it.  ``indices`` must be unique; a slot id outside the pool stores nothing.
+    """
+    if stream is None:
+        _native.store_kv_cache_mxfp4(kv_codes, kv_scales, indices, k, v, validate)
+        return
+    with _on_stream(stream, kv_codes):
+        _native.store_kv_cache_mxfp4(kv_codes, kv_scales, indices, k, v, validate)
+
+
+def load_kv_cache_mxfp4(kv_codes: torch.Tensor, kv_scales: torch.Tensor, indices: torch.Tensor, *,
+                        dtype: torch.dtype = torch.bfloat16, stream=None, validate: Optional[bool] = None):
+    """``(k, v)`` that slots ``indices`` of a pool of 4 bits hold, ``(length, num_kv_heads, head_dim)`` each: for moving rows
+    to another pool, or looking at what the rounding left.  Exact in bf16; float16 rounds what it cannot hold."""
+    if dtype not in (torch.bfloat16, torch.float16):
+        _fail("load_kv_cache_mxfp4", "dtype must be float16 or bfloat16")
+    if stream is None:
+        return _native.load_kv_cache_mxfp4(kv_codes, kv_scales, indices, dtype is torch.float16, validate)
+    with _on_stream(stream, kv_codes):
+        return _native.load_kv_cache_mxfp4(kv_codes, kv_scales, indices, dtype is torch.float16, validate)
+
+
+def qk_norm_rope_store_mxfp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
+                             k_weight: torch.Tensor, positions: torch.Tensor, out_loc: torch.Tensor,
+                             kv_codes: torch.Tensor, kv_scales: torch.Tensor, *, eps: float, rope_base: float,
+                             stream=None, validate: Optional[bool] = None) -> torch.Tensor:
+    """``qk_norm_rope_store`` into a pool of 4 bits; returns the rotated q.
+
+    Norm, weight and rotation are held in 32 bits and rounded once, to the result's bf16 or the pool's codes (``qk_norm_rope_store``
+    rounds to bf16 after each), and angles are made in 64 bits, so positions of any size are as good as small ones.
+    """
+    if stream is None:
+        return _native.qk_norm_rope_store_mxfp4(q, k, v, q_weight, k_weight, positions, out_loc, kv_codes,
+                                                kv_scales, eps, rope_base, validate)
+    with _on_stream(stream, q):
+        return _native.qk_norm_rope_store_mxfp4(q, k, v, q_weight, k_weight, positions, out_loc, kv_codes,
+                                                kv_scales, eps, rope_base, validate)
+
+
+def paged_decode_attention_mxfp4(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.Tensor,
+                                 kv_indptr: torch.Tensor, kv_indices: torch.Tensor, sm_scale: float, *,
+                                 stream=None, validate: Optional[bool] = None) -> torch.Tensor:
+    """``paged_decode_attention`` over a pool of 4 bits: ``q (batch, n_q, d)``, bf16 or float16, at most 16 q heads to a
+    kv head.  The pool's values are taken exactly; a request without keys gets zeros.  (float16: values beyond 98304, which only
+    a pool stored from bf16 has, come out as infinities.)"""
+    if stream is None:
+        return _native.paged_decode_attention_mxfp4(q, kv_codes, kv_scales, kv_indptr, kv_indices, sm_scale, validate)
+    with _on_stream(stream, q):
+        return _native.paged_decode_attention_mxfp4(q, kv_codes, kv_scales, kv_indptr, kv_indices, sm_scale, validate)
+
+
+def paged_prefill_attention_mxfp4(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.Tensor,
+                                  qo_indptr: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                                  prefix_lens: torch.Tensor, sm_scale: float, max_len_extend: int, *,
+                                  is_cross_attention: bool = False, sliding_window_size: int = 0,
+                                  stream=None, validate: Optional[bool] = None) -> torch.Tensor:
+    """``paged_prefill_attention`` over a pool of 4 bits (bf16), with the same masks: every key comes from the pool, the
+    queries' own among them, so how a prompt is cut into chunks does not change what it sees.
+
+    Short query blocks (verify, drafts) read the codes; longer ones have the listed rows unpacked into scratch memory first (4 * head_dim
+    * num_kv_heads bytes a listed key, one layer at a time) and run in the 16-bit pool's tile kernels."""
+    if stream is None:
+        return _native.paged_prefill_attention_mxfp4(q, kv_codes, kv_scales, qo_indptr, kv_indptr, kv_indices, prefix_lens, sm_scale,
+                                                     max_len_extend, is_cross_attention, sliding_window_size, validate)
+    with _on_stream(stream, q):
+        return _native.paged_prefill_attention_mxfp4(q, kv_codes, kv_scales, qo_indptr, kv_indptr, kv_indices, prefix_lens, sm_scale,
+                                                     max_len_extend, is_cross_attention, sliding_window_size, validate)
 
 
 def fast_compare_key(a: torch.Tensor, b: torch.Tensor) -> int:

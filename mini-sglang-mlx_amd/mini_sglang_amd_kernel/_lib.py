@@ -1,5 +1,5 @@
 """ctypes binding of ``libmsgl_paged_attention.so`` (the C ABI in ``include/msgl_paged_attention.h``,
-``include/msgl_radix_cache.h`` and ``include/msgl_state_pool.h``).
+``include/msgl_mxfp4_cache.h``, ``include/msgl_radix_cache.h`` and ``include/msgl_state_pool.h``).
 
 The library is built in-tree by ``mini-sglang-mlx_amd/build.py``; nothing here compiles at
 import time and nothing falls back to another implementation: a missing library is an
@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(_PKG_ROOT, "lib", "libmsgl_paged_attention.so")
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 
@@ -77,6 +78,24 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
          _i64, _i64, _i64, _i64, _i32, _i64, _vp, _sz, _vp]),
+    # include/msgl_mxfp4_cache.h (pool in 4 bits)
+    "msgl_store_kv_cache_mxfp4": (
+        ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "msgl_load_kv_cache_mxfp4": (
+        ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "msgl_qk_norm_rope_store_mxfp4": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _f64, _f64, _i32, _vp]),
+    "msgl_paged_decode_mxfp4_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "msgl_paged_decode_attention_mxfp4": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp]),
+    "msgl_paged_prefill_mxfp4_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "msgl_paged_prefill_attention_mxfp4": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _f32, _i32, _i32, _i32, _i32, _vp]),
     # include/msgl_state_pool.h (recurrent-state pool)
     "msgl_copy_state_slots": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
     # include/msgl_radix_cache.h (host-side prefix cache)
