@@ -12,12 +12,15 @@
 //                  block byte.  Four products take 8 dims of every block each, which is an order of the contraction like any other, and Q is
 //                  read in the same.
 //   O^T += V^T P^T mfma 16x16x32, dims on M.  Lane (r, g) reads dims 8 r .. 8 r + 7 of half h, one word, of each of the 8 keys of group g, and turns the 8 x 8 values
-//                  over after the conversion.  Row 4 a + i of the two products of S^T is key 8 a + i and 8 a + 4 + i, so the
+//                  over after the conversion.  Row 4 a + i of product u of S^T is key 8 a + of_group(4 u + i), so the
 //                  weights of group g's keys are the ones that its lanes hold.
 // The conversion multiplies by the block's factor on the way (one instruction for two values), so codes cost what 16-bit values would.
 // Weights are rounded to the type of q for the second product (half a step, 2^-8 and 2^-11 of a weight, as the 16-bit pool's
 // kernels do); scores, sums and accumulators have 32 bits, and so do the partials.
+#include <type_traits>
+
 #include "mxfp4.h"
+#include "prefill_tile_common.h"
 #include "splitkv_stream.h"
 
 namespace msgl {
@@ -93,6 +96,31 @@ __device__ __forceinline__ void start_mx_columns(const SplitKvParams& p, const R
   }
 }
 
+// Where the 32 keys of a tile lie in a wave's stage of LDS, and who takes them to registers.  A load moves 1 KiB: whole slots of a head (8 at
+// head_dim 128, 4 at 256), 16 bytes a lane, which come to lie one behind the other; the 16-byte pieces of a row are exchanged among
+// themselves so that the 16 lanes of a read find theirs in different banks.
+//   row(key), piece c at place c ^ turn(key) of its row
+// Keys of a lane group's 8, in the order n = 4 u + i in which S^T has them (row 4 a + i of product u): of_group(n).
+template <int D>
+struct Place;
+template <>
+struct Place<128> {
+  static constexpr int kLoads = 4, kScaleLoads = 1, kLanes = 8;  // lanes to a row in a load
+  static __device__ __forceinline__ constexpr int of_group(int n) { return (n & 1) + 4 * ((n >> 1) & 1) + 2 * (n >> 2); }
+  // load u, lanes 8 j ..: key 4 j + u
+  static __device__ __forceinline__ int key(int u, int j) { return 4 * j + u; }
+  static __device__ __forceinline__ constexpr int row(int key) { return 8 * (key & 3) + (key >> 2); }
+  static __device__ __forceinline__ constexpr int turn(int key) { return ((key >> 3) & 3) | ((key & 1) << 2); }
+};
+template <>
+struct Place<256> {
+  static constexpr int kLoads = 8, kScaleLoads = 2, kLanes = 16;
+  static __device__ __forceinline__ constexpr int of_group(int n) { return n; }
+  static __device__ __forceinline__ int key(int u, int j) { return 8 * j + u; }
+  static __device__ __forceinline__ constexpr int row(int key) { return 4 * (key & 7) + (key >> 3); }
+  static __device__ __forceinline__ constexpr int turn(int key) { return (key >> 3) | ((key & 3) << 2); }
+};
+
 // Keys tb .. tb + 31 for the columns in `c_`
 template <int D, int NCT, bool F16>
 __device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const MxTile<D>& t, int tb, MxColumns<D, NCT>& c_) {
@@ -118,13 +146,13 @@ __device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const Mx
   u32x4_t pb[NCT];
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct) {
-    float x[8];  // of key tb + 8 g + n
+    float x[8];  // of key tb + 8 g + of_group(n)
 #pragma unroll
     for (int n = 0; n < 8; ++n) x[n] = s[n >> 2][ct][n & 3] * p.scale_log2e;
     if (need_mask) {
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const int key = tb + 8 * g + n;
+        const int key = tb + 8 * g + Place<D>::of_group(n);
         if (key < c_.lo[ct] || key > c_.hi[ct]) x[n] = kNegInf;
       }
     }
@@ -169,36 +197,106 @@ __device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const Mx
   }
 }
 
-// Keys [t_begin, t_end) of request `r`, in order, for the columns in `c_`
-template <int D, int NCT, bool F16>
-__device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const ReqInfo& r, int kvh, int t_begin, int t_end, MxColumns<D, NCT>& c_) {
-  const int t16 = lane_id() & 15, g = lane_id() >> 4;
+// A wave's LDS: stages of codes and block bytes, and the slot ids of tiles to come.
+template <int D>
+struct WaveLds {
+  static constexpr int kAhead = D == 128 ? 3 : 1, kStages = kAhead + 1;    // tiles on their way while one is computed
+  static constexpr int kIdsAhead = kAhead + 1, kIdTiles = 2 * kStages;  // ids are asked for so many tiles before their tile is
+  static_assert((kStages & (kStages - 1)) == 0 && kIdTiles >= kAhead + kIdsAhead + 1);
+  static constexpr int kCodes = 32 * D, kScales = 32 * (D / 16), kStage = kCodes + kScales, kIds = kStages * kStage;
+  unsigned char bytes[kIds + kIdTiles * 256];
+};
+
+// At most N loads of the wave under way, and none of its reads of LDS: the stage that the next loads write has been read.
+template <int N>
+__device__ __forceinline__ void wait_tile() {
+  static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit field");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+
+// Keys [t_begin, t_end) of request `r`, in order, for the columns in `c_`; `lds`: the wave's own, so nobody else is waited for.
+// Everything comes by loads that write LDS, of which the compiler knows nothing: tile i is there when no more of them than those issued
+// behind its last are under way.  Each iteration issues the same number, in the same order: codes and block bytes of the tile kAhead on, ids of the tile kAhead +
+// kIdsAhead on.  Keys past the end are the last one again, and masked.
+template <int D, int NCT, bool F16, bool WIDE>
+__device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const ReqInfo& r, int kvh, int t_begin, int t_end, unsigned char* lds,
+                                               MxColumns<D, NCT>& c_) {
+  using P = Place<D>;
+  using L = WaveLds<D>;
+  constexpr int kAhead = L::kAhead, kStages = L::kStages, kIdsAhead = L::kIdsAhead, kIdTiles = L::kIdTiles;
+  constexpr int kIssued = P::kLoads + P::kScaleLoads + 1;
+  constexpr int kScaleWords = D / 64;  // of 4 bytes, of a key
+  using Offset = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
+  const int lane = lane_id(), t16 = lane & 15, g = lane >> 4, a = t16 >> 2, i = t16 & 3;
   const unsigned char* codes = reinterpret_cast<const unsigned char*>(p.k_cache) + kvh * D;
   const unsigned char* scales = reinterpret_cast<const unsigned char*>(p.v_cache) + kvh * (D / 16);
-  const int32_t* idx = p.kv_indices + r.kv_start;
-  auto slot_of = [&](int key) { return (int64_t)min((uint32_t)idx[min(key, t_end - 1)], p.max_slot); };
-  for (int tb = t_begin; tb < t_end; tb += 32) {
+  const int32_t* idx = p.kv_indices + r.kv_start + t_begin;
+  const int last = t_end - t_begin - 1, n_tiles = (last >> 5) + 1;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)MSGL_LDS_PTR(unsigned char, lds));
+  const auto shared = MSGL_LDS_PTR(unsigned char, lds);
+  const uint32_t codes_stride = (uint32_t)p.k_stride0, scales_stride = (uint32_t)p.v_stride0;
+  auto offset = [](uint32_t slot, uint32_t stride) { return (Offset)slot * stride; };
+
+  const int j = lane / P::kLanes, piece = lane % P::kLanes;
+  auto send_ids = [&](int tile) {
+    lds_direct_b32(lds0 + L::kIds + (uint32_t)(tile & (kIdTiles - 1)) * 256u, idx, (uint32_t)min(tile * 32 + (lane & 31), last) * 4u);
+  };
+  auto send_tile = [&](int tile) {
+    const uint32_t stage = lds0 + (uint32_t)(tile & (kStages - 1)) * L::kStage;
+    const auto ids = shared + L::kIds + (tile & (kIdTiles - 1)) * 256;
+    uint32_t slot[P::kLoads];
+#pragma unroll
+    for (int q = 0; q < P::kLoads; q += 4) {
+      const u32x4_t four = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(ids + P::key(q, j) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) slot[q + e] = min(four[e], p.max_slot);
+    }
+    uint32_t scale_slot[P::kScaleLoads];
+#pragma unroll
+    for (int q = 0; q < P::kScaleLoads; ++q)
+      scale_slot[q] = min(*reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(ids + ((64 / kScaleWords) * q + lane / kScaleWords) * 4), p.max_slot);
+#pragma unroll
+    for (int u = 0; u < P::kLoads; ++u)
+      lds_direct_b128(stage + u * 1024u, codes, offset(slot[u], codes_stride) + (uint32_t)((piece ^ P::turn(P::key(u, j))) * 16));
+#pragma unroll
+    for (int q = 0; q < P::kScaleLoads; ++q)
+      lds_direct_b32(stage + L::kCodes + q * 256u, scales, offset(scale_slot[q], scales_stride) + (uint32_t)(lane % kScaleWords) * 4u);
+  };
+  for (int tile = 0; tile < kIdsAhead; ++tile) send_ids(tile);
+  wait_all_vm();
+#pragma unroll
+  for (int tile = 0; tile < kAhead; ++tile) {
+    send_tile(tile);
+    send_ids(tile + kIdsAhead);
+  }
+  for (int tile = 0; tile < n_tiles; ++tile) {
+    wait_tile<(kAhead - 1) * kIssued + 1>();
+    send_tile(tile + kAhead);
+    send_ids(tile + kAhead + kIdsAhead);
+    const auto at = shared + (tile & (kStages - 1)) * L::kStage;
     MxTile<D> t;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int64_t slot = slot_of(tb + 8 * (t16 >> 2) + 4 * u + (t16 & 3));
+      const int key = 8 * a + P::of_group(i) + (P::of_group(4 * u) - P::of_group(0));
 #pragma unroll
       for (int h = 0; h < D / 128; ++h) {
-        t.k[h][u] = ld_global_b128(codes + slot * p.k_stride0 + (4 * h + g) * 16);
-        t.k_byte[h][u] = scales[slot * p.v_stride0 + 4 * h + g];
+        t.k[h][u] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(at + P::row(key) * D + ((4 * h + g) ^ P::turn(key)) * 16);
+        t.k_byte[h][u] = at[L::kCodes + key * (D / 16) + 4 * h + g];
       }
     }
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const int64_t slot = slot_of(tb + 8 * g + n);
+      const int key = 8 * g + P::of_group(n);
 #pragma unroll
       for (int h = 0; h < D / 128; ++h) {
-        t.v[h][n] = *reinterpret_cast<const uint32_t*>(codes + slot * p.k_stride0 + D / 2 + h * 64 + t16 * 4);
-        t.v_byte[h][n] = scales[slot * p.v_stride0 + D / 32 + 4 * h + (t16 >> 2)];
+        t.v[h][n] = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(at + P::row(key) * D + ((D / 32 + 4 * h + a) ^ P::turn(key)) * 16 + i * 4);
+        t.v_byte[h][n] = at[L::kCodes + key * (D / 16) + D / 32 + 4 * h + a];
       }
     }
-    compute_mx_tile<D, NCT, F16>(p, t, tb, c_);
+    compute_mx_tile<D, NCT, F16>(p, t, t_begin + tile * 32, c_);
   }
+  wait_all_vm();  // what is still under way writes LDS that the next keys want
 }
 
 // A request's share is done: its rows, if the segment held all of it, else its partial.
@@ -246,14 +344,18 @@ __device__ __forceinline__ void leave_share(const SplitKvParams& p, const ReqInf
   }
 }
 
-template <int D, int NCT, bool F16>
-__global__ __launch_bounds__(256) void mxfp4_attention_kernel(SplitKvParams p) {
+template <int D, int NCT, bool F16, bool WIDE, int NW>
+__global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1) void mxfp4_attention_kernel(SplitKvParams p) {
+  __shared__ __attribute__((aligned(256))) WaveLds<D> lds[NW];
   const int seg = blockIdx.x / p.head_groups;
-  const int kvh = (blockIdx.x - seg * p.head_groups) * p.nwh + (threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = (blockIdx.x - seg * p.head_groups) * p.nwh + wave;
   int seg_len, total, b, vs;
   if (!locate_segment(p, seg, &seg_len, &total, &b, &vs)) return;
   b = __builtin_amdgcn_readfirstlane(b);
   vs = __builtin_amdgcn_readfirstlane(vs);
+  seg_len = __builtin_amdgcn_readfirstlane(seg_len);
+  total = __builtin_amdgcn_readfirstlane(total);
   int vpos = seg * seg_len;
   const int seg_end = min(vpos + seg_len, total);
   while (vpos < seg_end && b < p.batch) {
@@ -275,10 +377,22 @@ __global__ __launch_bounds__(256) void mxfp4_attention_kernel(SplitKvParams p) {
     }
     MxColumns<D, NCT> c_;
     start_mx_columns<D, NCT, F16>(p, r, kvh, t_end, c_);
-    attend_mx_keys<D, NCT, F16>(p, r, kvh, t_begin, t_end, c_);
+    attend_mx_keys<D, NCT, F16, WIDE>(p, r, kvh, t_begin, t_end, lds[wave].bytes, c_);
     leave_share<D, NCT, F16>(p, r, seg, b, kvh, t_begin == r.lo && t_end == r.hi, c_);
     vpos += t_end - t_begin;
   }
+}
+
+template <int D, int NCT, bool F16>
+int launch_width(const SplitKvParams& p, bool wide, hipStream_t stream) {
+  auto launch = [&](auto kernel) { return launch_kernel(kernel, dim3((unsigned)(p.n_seg * p.head_groups)), dim3(64 * p.nwh), stream, p); };
+  auto heads = [&](auto w) {
+    constexpr bool WIDE = decltype(w)::value;
+    return p.nwh == 4   ? launch(mxfp4_attention_kernel<D, NCT, F16, WIDE, 4>)
+           : p.nwh == 2 ? launch(mxfp4_attention_kernel<D, NCT, F16, WIDE, 2>)
+                        : launch(mxfp4_attention_kernel<D, NCT, F16, WIDE, 1>);
+  };
+  return wide ? heads(std::true_type{}) : heads(std::false_type{});
 }
 
 constexpr int kMinSegment = 64;
@@ -332,19 +446,16 @@ int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_lse = reinterpret_cast<float*>(ws + (size_t)rows * d * sizeof(float));
   p.req_items = reinterpret_cast<int32_t*>(ws + (size_t)rows * (d + 1) * sizeof(float));
-  auto launch = [&](auto kernel) {
-    return launch_kernel(kernel, dim3((unsigned)(p.n_seg * p.head_groups)), dim3(64 * p.nwh), stream, p);
-  };
   const int nct = (int)((cols + 15) / 16);
-  int rc;
   if (a.f16 && nct > 1) return MSGL_ERR_DTYPE;
-  if (d == 128)
-    rc = launch(a.f16      ? mxfp4_attention_kernel<128, 1, true>
-                : nct == 1 ? mxfp4_attention_kernel<128, 1, false>
-                : nct == 2 ? mxfp4_attention_kernel<128, 2, false>
-                           : mxfp4_attention_kernel<128, 4, false>);
-  else
-    rc = launch(a.f16 ? mxfp4_attention_kernel<256, 1, true> : nct == 1 ? mxfp4_attention_kernel<256, 1, false> : mxfp4_attention_kernel<256, 2, false>);
+  const bool wide = (uint64_t)a.pool.num_slots * (uint64_t)std::max(a.pool.codes_stride0, a.pool.scales_stride0) >= (1ull << 32);
+  const int rc = d == 128 ? (a.f16      ? launch_width<128, 1, true>(p, wide, stream)
+                             : nct == 1 ? launch_width<128, 1, false>(p, wide, stream)
+                             : nct == 2 ? launch_width<128, 2, false>(p, wide, stream)
+                                        : launch_width<128, 4, false>(p, wide, stream))
+                          : (a.f16      ? launch_width<256, 1, true>(p, wide, stream)
+                             : nct == 1 ? launch_width<256, 1, false>(p, wide, stream)
+                                        : launch_width<256, 2, false>(p, wide, stream));
   return rc != MSGL_OK ? rc : launch_fp32_merge(p, d, stream);
 }
 

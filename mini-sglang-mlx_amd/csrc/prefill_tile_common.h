@@ -36,6 +36,13 @@ __device__ __forceinline__ void lds_direct_b32(uint32_t lds_addr, const void* sa
                : "s"(lds_addr), "v"(voff), "s"(saddr)
                : "memory");
 }
+__device__ __forceinline__ void lds_direct_b32(uint32_t lds_addr, const void* saddr, uint64_t voff) {
+  const unsigned char* a = static_cast<const unsigned char*>(saddr) + voff;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"(lds_addr), "v"(a)
+               : "memory");
+}
 // s_waitcnt vmcnt(0) (expcnt and lgkmcnt fields left at their maxima).  Issued through the
 // builtin so that the compiler's own wait bookkeeping sees it.
 __device__ __forceinline__ void wait_all_vm() {
