@@ -26,12 +26,17 @@
 namespace msgl {
 namespace {
 
+struct MxParams : SplitKvParams {
+  int32_t negate;  // scale_log2e is positive: with a scale below zero (-1) the scores of -q count, with none (1) those of zeros
+};
+
 template <int D, int NCT>
 struct MxColumns {
   u32x4_t q[NCT][D / 32];      // [4 h + c]: dims 128 h + 32 g + 8 c ..
   int lo[NCT], hi[NCT];        // first and last visible key of this lane's column in each tile of 16
   int all_lo, all_hi;          // keys inside are visible to every column
-  float m[NCT], l[NCT];        // running maximum (base 2); this lane's part of the sum
+  float m[NCT], l[NCT];        // what the weights are relative to (base 2; 0 before the first key); this lane's part of their sum
+  float top[NCT];              // m, or -infinity before the first key
   f32x4_t o[NCT][D / 128][8];  // [h][n][i]: dim 128 h + 8 (4 g + i) + n
 };
 
@@ -54,7 +59,7 @@ template <bool F16>
 constexpr float kBack = F16 ? 2.f : 1.f;
 
 template <int D, int NCT, bool F16>
-__device__ __forceinline__ void start_mx_columns(const SplitKvParams& p, const ReqInfo& r, int kvh, int t_end, MxColumns<D, NCT>& c_) {
+__device__ __forceinline__ void start_mx_columns(const MxParams& p, const ReqInfo& r, int kvh, int t_end, MxColumns<D, NCT>& c_) {
   const int t16 = lane_id() & 15, g = lane_id() >> 4;
   const int ncols = r.q_len * p.group;
   int all_lo = 0, all_hi = 0x7fffffff;
@@ -69,6 +74,7 @@ __device__ __forceinline__ void start_mx_columns(const SplitKvParams& p, const R
     for (int s = 0; s < D / 32; ++s) {
       c_.q[ct][s] = u32x4_t{0u, 0u, 0u, 0u};
       if (valid) c_.q[ct][s] = ld_global_b128(qrow + (s >> 2) * 128 + (s & 3) * 8);
+      if (p.negate != 0) c_.q[ct][s] = p.negate < 0 ? c_.q[ct][s] ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
     }
     const int qpos = r.prefix + qi;
     int lo = (p.window > 0) ? qpos - p.window + 1 : 0;
@@ -87,7 +93,8 @@ __device__ __forceinline__ void start_mx_columns(const SplitKvParams& p, const R
   c_.all_hi = __builtin_amdgcn_readfirstlane(~row_max16(~all_hi));
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct) {
-    c_.m[ct] = kNegInf;
+    c_.m[ct] = 0.f;
+    c_.top[ct] = kNegInf;
     c_.l[ct] = 0.f;
 #pragma unroll
     for (int h = 0; h < D / 128; ++h)
@@ -111,6 +118,14 @@ struct Place<128> {
   static __device__ __forceinline__ int key(int u, int j) { return 4 * j + u; }
   static __device__ __forceinline__ constexpr int row(int key) { return 8 * (key & 3) + (key >> 2); }
   static __device__ __forceinline__ constexpr int turn(int key) { return ((key >> 3) & 3) | ((key & 1) << 2); }
+  // What a lane reads, as the sum of its own part and one of the instruction: lane (4 a + i, g) piece g of key 8 a + of_group(4 u + i), ...
+  static __device__ __forceinline__ int k_lane(int a, int i, int g) { return (8 * (i & 1) + 2 * a + (i >> 1)) * 128 + ((g ^ a) + 4 * (i & 1)) * 16; }
+  static __device__ __forceinline__ int k_lane_h(int a, int i, int g) { return k_lane(a, i, g); }
+  static __device__ __forceinline__ constexpr int k_of(int u) { return 16 * 128 * u; }
+  static __device__ __forceinline__ int k_byte(int a, int i, int g) { return (8 * a + of_group(i)) * 8 + g; }
+  // ... and word 4 a + i of V of key 8 g + of_group(n)
+  static __device__ __forceinline__ int v_lane(int a, int i, int g) { return 2 * g * 128 + (a ^ g) * 16 + i * 4; }
+  static __device__ __forceinline__ constexpr int v_of(int n, int) { return (8 * ((n & 1) + 2 * (n >> 2)) + ((n >> 1) & 1)) * 128 + (n & 1 ? 0 : 64); }
 };
 template <>
 struct Place<256> {
@@ -119,7 +134,20 @@ struct Place<256> {
   static __device__ __forceinline__ int key(int u, int j) { return 8 * j + u; }
   static __device__ __forceinline__ constexpr int row(int key) { return 4 * (key & 7) + (key >> 3); }
   static __device__ __forceinline__ constexpr int turn(int key) { return (key >> 3) | ((key & 3) << 2); }
+  static __device__ __forceinline__ int k_lane(int a, int i, int g) { return (4 * i + a) * 256 + (4 * i + (g ^ a)) * 16; }
+  static __device__ __forceinline__ int k_lane_h(int a, int i, int g) { return (4 * i + a) * 256 + (4 * (i ^ 1) + (g ^ a)) * 16; }
+  static __device__ __forceinline__ constexpr int k_of(int u) { return 16 * 256 * u; }
+  static __device__ __forceinline__ int k_byte(int a, int i, int g) { return (8 * a + i) * 16 + g; }
+  static __device__ __forceinline__ int v_lane(int a, int i, int g) { return g * 256 + (a ^ g) * 16 + i * 4; }
+  static __device__ __forceinline__ constexpr int v_of(int n, int h) { return 4 * n * 256 + ((2 + h) ^ (n & 3)) * 64; }
 };
+
+// sum + both weights of a pair
+template <bool F16>
+__device__ __forceinline__ float add_weights(uint32_t pair, float sum) {
+  if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pair), f16x2_t{(_Float16)1.f, (_Float16)1.f}, sum, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), kOnes, sum, false);
+}
 
 // Keys tb .. tb + 31 for the columns in `c_`
 template <int D, int NCT, bool F16>
@@ -148,7 +176,7 @@ __device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const Mx
   for (int ct = 0; ct < NCT; ++ct) {
     float x[8];  // of key tb + 8 g + of_group(n)
 #pragma unroll
-    for (int n = 0; n < 8; ++n) x[n] = s[n >> 2][ct][n & 3] * p.scale_log2e;
+    for (int n = 0; n < 8; ++n) x[n] = s[n >> 2][ct][n & 3];
     if (need_mask) {
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
@@ -156,26 +184,26 @@ __device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const Mx
         if (key < c_.lo[ct] || key > c_.hi[ct]) x[n] = kNegInf;
       }
     }
-    float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    mx = max_across<32>(max_across<16>(mx));
-    const float m_new = fmaxf(c_.m[ct], mx);
-    const float m_safe = (m_new == kNegInf) ? 0.f : m_new;
-    const float alpha = fast_exp2(c_.m[ct] - m_safe);
-    c_.m[ct] = m_new;
-    float psum = 0.f;
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      x[n] = fast_exp2(x[n] - m_safe);
-      psum += x[n];
-    }
-    c_.l[ct] = c_.l[ct] * alpha + psum;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pb[ct][i] = pack_16x2<F16>(x[2 * i], x[2 * i + 1]);
-    if (__any(alpha != 1.0f)) {
+    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * p.scale_log2e;
+    // The reference moves only where a score is far beyond it: weights up to 2^kLazy are as exact as those up to 1
+    if (__any(mx > c_.top[ct] + kLazy)) {
+      const float top = fmaxf(c_.top[ct], max_across<32>(max_across<16>(mx)));
+      const float m = top == kNegInf ? 0.f : top;
+      const float alpha = fast_exp2(c_.top[ct] - m);
+      c_.top[ct] = top;
+      c_.m[ct] = m;
+      c_.l[ct] *= alpha;
 #pragma unroll
       for (int h = 0; h < D / 128; ++h)
 #pragma unroll
         for (int n = 0; n < 8; ++n) c_.o[ct][h][n] *= alpha;
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) x[n] = fast_exp2(__builtin_fmaf(x[n], p.scale_log2e, -c_.m[ct]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pb[ct][i] = pack_16x2<F16>(x[2 * i], x[2 * i + 1]);
+      c_.l[ct] = add_weights<F16>(pb[ct][i], c_.l[ct]);  // the ones that multiply V
     }
   }
 #pragma unroll
@@ -219,7 +247,7 @@ __device__ __forceinline__ void wait_tile() {
 // Everything comes by loads that write LDS, of which the compiler knows nothing: tile i is there when no more of them than those issued
 // behind its last are under way.  Each iteration issues the same number, in the same order: codes and block bytes of the tile kAhead on, ids of the tile kAhead +
 // kIdsAhead on.  Keys past the end are the last one again, and masked.
-template <int D, int NCT, bool F16, bool WIDE>
+template <int D, int NCT, bool F16, int WALK>
 __device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const ReqInfo& r, int kvh, int t_begin, int t_end, unsigned char* lds,
                                                MxColumns<D, NCT>& c_) {
   using P = Place<D>;
@@ -227,7 +255,7 @@ __device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const Req
   constexpr int kAhead = L::kAhead, kStages = L::kStages, kIdsAhead = L::kIdsAhead, kIdTiles = L::kIdTiles;
   constexpr int kIssued = P::kLoads + P::kScaleLoads + 1;
   constexpr int kScaleWords = D / 64;  // of 4 bytes, of a key
-  using Offset = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
+  using Offset = typename std::conditional<(WALK & kWide) != 0, uint64_t, uint32_t>::type;
   const int lane = lane_id(), t16 = lane & 15, g = lane >> 4, a = t16 >> 2, i = t16 & 3;
   const unsigned char* codes = reinterpret_cast<const unsigned char*>(p.k_cache) + kvh * D;
   const unsigned char* scales = reinterpret_cast<const unsigned char*>(p.v_cache) + kvh * (D / 16);
@@ -236,7 +264,10 @@ __device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const Req
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)MSGL_LDS_PTR(unsigned char, lds));
   const auto shared = MSGL_LDS_PTR(unsigned char, lds);
   const uint32_t codes_stride = (uint32_t)p.k_stride0, scales_stride = (uint32_t)p.v_stride0;
-  auto offset = [](uint32_t slot, uint32_t stride) { return (Offset)slot * stride; };
+  auto offset = [](uint32_t slot, uint32_t stride) -> Offset {
+    if constexpr (WALK & kWide) return (uint64_t)slot * stride;
+    else return __umul24(slot, stride);  // both below 2^24 here
+  };
 
   const int j = lane / P::kLanes, piece = lane % P::kLanes;
   auto send_ids = [&](int tile) {
@@ -257,8 +288,11 @@ __device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const Req
     for (int q = 0; q < P::kScaleLoads; ++q)
       scale_slot[q] = min(*reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(ids + ((64 / kScaleWords) * q + lane / kScaleWords) * 4), p.max_slot);
 #pragma unroll
-    for (int u = 0; u < P::kLoads; ++u)
-      lds_direct_b128(stage + u * 1024u, codes, offset(slot[u], codes_stride) + (uint32_t)((piece ^ P::turn(P::key(u, j))) * 16));
+    for (int u = 0; u < P::kLoads; ++u) {
+      const Offset from = offset(slot[u], codes_stride) + (uint32_t)((piece ^ P::turn(P::key(u, j))) * 16);
+      if constexpr (WALK & kStream) lds_stream_b128(stage + u * 1024u, codes, from);
+      else lds_direct_b128(stage + u * 1024u, codes, from);
+    }
 #pragma unroll
     for (int q = 0; q < P::kScaleLoads; ++q)
       lds_direct_b32(stage + L::kCodes + q * 256u, scales, offset(scale_slot[q], scales_stride) + (uint32_t)(lane % kScaleWords) * 4u);
@@ -275,25 +309,23 @@ __device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const Req
     send_tile(tile + kAhead);
     send_ids(tile + kAhead + kIdsAhead);
     const auto at = shared + (tile & (kStages - 1)) * L::kStage;
+    const auto k_at = at + P::k_lane(a, i, g), v_at = at + P::v_lane(a, i, g);
+    const auto kb_at = at + L::kCodes + P::k_byte(a, i, g), vb_at = at + L::kCodes + 8 * g * (D / 16) + D / 32 + a;
     MxTile<D> t;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int key = 8 * a + P::of_group(i) + (P::of_group(4 * u) - P::of_group(0));
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int h = 0; h < D / 128; ++h) {
-        t.k[h][u] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(at + P::row(key) * D + ((4 * h + g) ^ P::turn(key)) * 16);
-        t.k_byte[h][u] = at[L::kCodes + key * (D / 16) + 4 * h + g];
+        t.k[h][u] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>((h == 0 ? k_at : at + P::k_lane_h(a, i, g)) + P::k_of(u));
+        t.k_byte[h][u] = kb_at[(P::of_group(4 * u) - P::of_group(0)) * (D / 16) + 4 * h];
       }
-    }
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int key = 8 * g + P::of_group(n);
+    for (int n = 0; n < 8; ++n)
 #pragma unroll
       for (int h = 0; h < D / 128; ++h) {
-        t.v[h][n] = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(at + P::row(key) * D + ((D / 32 + 4 * h + a) ^ P::turn(key)) * 16 + i * 4);
-        t.v_byte[h][n] = at[L::kCodes + key * (D / 16) + D / 32 + 4 * h + a];
+        t.v[h][n] = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(v_at + P::v_of(n, h));
+        t.v_byte[h][n] = vb_at[P::of_group(n) * (D / 16) + 4 * h];
       }
-    }
     compute_mx_tile<D, NCT, F16>(p, t, t_begin + tile * 32, c_);
   }
   wait_all_vm();  // what is still under way writes LDS that the next keys want
@@ -344,8 +376,8 @@ __device__ __forceinline__ void leave_share(const SplitKvParams& p, const ReqInf
   }
 }
 
-template <int D, int NCT, bool F16, bool WIDE, int NW>
-__global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1) void mxfp4_attention_kernel(SplitKvParams p) {
+template <int D, int NCT, bool F16, int WALK, int NW>
+__global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1) void mxfp4_attention_kernel(MxParams p) {
   __shared__ __attribute__((aligned(256))) WaveLds<D> lds[NW];
   const int seg = blockIdx.x / p.head_groups;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -377,22 +409,25 @@ __global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1
     }
     MxColumns<D, NCT> c_;
     start_mx_columns<D, NCT, F16>(p, r, kvh, t_end, c_);
-    attend_mx_keys<D, NCT, F16, WIDE>(p, r, kvh, t_begin, t_end, lds[wave].bytes, c_);
+    attend_mx_keys<D, NCT, F16, WALK>(p, r, kvh, t_begin, t_end, lds[wave].bytes, c_);
     leave_share<D, NCT, F16>(p, r, seg, b, kvh, t_begin == r.lo && t_end == r.hi, c_);
     vpos += t_end - t_begin;
   }
 }
 
 template <int D, int NCT, bool F16>
-int launch_width(const SplitKvParams& p, bool wide, hipStream_t stream) {
+int launch_walk(const MxParams& p, hipStream_t stream) {
   auto launch = [&](auto kernel) { return launch_kernel(kernel, dim3((unsigned)(p.n_seg * p.head_groups)), dim3(64 * p.nwh), stream, p); };
   auto heads = [&](auto w) {
-    constexpr bool WIDE = decltype(w)::value;
-    return p.nwh == 4   ? launch(mxfp4_attention_kernel<D, NCT, F16, WIDE, 4>)
-           : p.nwh == 2 ? launch(mxfp4_attention_kernel<D, NCT, F16, WIDE, 2>)
-                        : launch(mxfp4_attention_kernel<D, NCT, F16, WIDE, 1>);
+    constexpr int WALK = decltype(w)::value;
+    return p.nwh == 4   ? launch(mxfp4_attention_kernel<D, NCT, F16, WALK, 4>)
+           : p.nwh == 2 ? launch(mxfp4_attention_kernel<D, NCT, F16, WALK, 2>)
+                        : launch(mxfp4_attention_kernel<D, NCT, F16, WALK, 1>);
   };
-  return wide ? heads(std::true_type{}) : heads(std::false_type{});
+  return p.walk == (kStream | kWide) ? heads(std::integral_constant<int, kStream | kWide>{})
+         : p.walk == kStream         ? heads(std::integral_constant<int, kStream>{})
+         : p.walk == kWide           ? heads(std::integral_constant<int, kWide>{})
+                                     : heads(std::integral_constant<int, kNarrow>{});
 }
 
 constexpr int kMinSegment = 64;
@@ -413,7 +448,7 @@ size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t total_kv, int64_t 
 int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   const int64_t n_kv = a.pool.n_kv, d = a.pool.head_dim, cols = a.n_q / n_kv * a.max_len_extend;
   if (cols < 1 || cols > mxfp4_max_columns(d)) return MSGL_ERR_SHAPE;
-  SplitKvParams p{};
+  MxParams p{};
   p.q = static_cast<const uint16_t*>(a.q);
   p.k_cache = static_cast<const uint16_t*>(a.pool.codes);   // as bytes, strides too
   p.v_cache = static_cast<const uint16_t*>(a.pool.scales);
@@ -440,7 +475,8 @@ int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   p.is_cross = a.is_cross;
   p.window = a.window;
   p.max_slot = (uint32_t)(a.pool.num_slots - 1);
-  p.scale_log2e = a.sm_scale * kLog2e * (a.f16 ? 2.f : 1.f);
+  p.negate = a.sm_scale < 0.f ? -1 : a.sm_scale == 0.f ? 1 : 0;
+  p.scale_log2e = a.sm_scale == 0.f ? 1.f : fabsf(a.sm_scale) * kLog2e * (a.f16 ? 2.f : 1.f);
   const int64_t rows = ((int64_t)p.n_seg + a.batch) * n_kv * cols;
   char* ws = static_cast<char*>(a.workspace);
   p.part_o = reinterpret_cast<float*>(ws);
@@ -448,14 +484,17 @@ int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   p.req_items = reinterpret_cast<int32_t*>(ws + (size_t)rows * (d + 1) * sizeof(float));
   const int nct = (int)((cols + 15) / 16);
   if (a.f16 && nct > 1) return MSGL_ERR_DTYPE;
-  const bool wide = (uint64_t)a.pool.num_slots * (uint64_t)std::max(a.pool.codes_stride0, a.pool.scales_stride0) >= (1ull << 32);
-  const int rc = d == 128 ? (a.f16      ? launch_width<128, 1, true>(p, wide, stream)
-                             : nct == 1 ? launch_width<128, 1, false>(p, wide, stream)
-                             : nct == 2 ? launch_width<128, 2, false>(p, wide, stream)
-                                        : launch_width<128, 4, false>(p, wide, stream))
-                          : (a.f16      ? launch_width<256, 1, true>(p, wide, stream)
-                             : nct == 1 ? launch_width<256, 1, false>(p, wide, stream)
-                                        : launch_width<256, 2, false>(p, wide, stream));
+  const int64_t stride = std::max(a.pool.codes_stride0, a.pool.scales_stride0);
+  const bool wide = a.pool.num_slots > 1 << 24 || stride >= 1 << 24 || (uint64_t)a.pool.num_slots * (uint64_t)stride >= (1ull << 32);
+  const int64_t keys = visible_keys(a.batch, a.total_kv, a.window, a.max_len_extend, a.is_cross != 0);
+  p.walk = (wide ? kWide : kNarrow) | (streams(keys * n_kv * (d + d / 16)) ? kStream : kNarrow);
+  const int rc = d == 128 ? (a.f16      ? launch_walk<128, 1, true>(p, stream)
+                             : nct == 1 ? launch_walk<128, 1, false>(p, stream)
+                             : nct == 2 ? launch_walk<128, 2, false>(p, stream)
+                                        : launch_walk<128, 4, false>(p, stream))
+                          : (a.f16      ? launch_walk<256, 1, true>(p, stream)
+                             : nct == 1 ? launch_walk<256, 1, false>(p, stream)
+                                        : launch_walk<256, 2, false>(p, stream));
   return rc != MSGL_OK ? rc : launch_fp32_merge(p, d, stream);
 }
 

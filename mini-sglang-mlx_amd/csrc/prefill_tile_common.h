@@ -29,6 +29,20 @@ __device__ __forceinline__ void lds_direct_b128(uint32_t lds_addr, const void* s
                : "s"(lds_addr), "v"(a)
                : "memory");
 }
+// The same past the caches (ld_stream_b128)
+__device__ __forceinline__ void lds_stream_b128(uint32_t lds_addr, const void* saddr, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+               :
+               : "s"(lds_addr), "v"(voff), "s"(saddr)
+               : "memory");
+}
+__device__ __forceinline__ void lds_stream_b128(uint32_t lds_addr, const void* saddr, uint64_t voff) {
+  const unsigned char* a = static_cast<const unsigned char*>(saddr) + voff;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+               :
+               : "s"(lds_addr), "v"(a)
+               : "memory");
+}
 // 64 lanes x 4 bytes: lane l's dword at `saddr + voff` lands at LDS byte lds_addr + 4 l.
 __device__ __forceinline__ void lds_direct_b32(uint32_t lds_addr, const void* saddr, uint32_t voff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"

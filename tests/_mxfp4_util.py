@@ -33,15 +33,15 @@ def indptr(lens, start=0):
 def tolerance(spread, score, out, d, dtype=torch.bfloat16, cut=False):
     """How far a result may be off its definition in 64 bits, entry by entry.
 
-    With A = sum_j w_j |v_j|: weights that are rounded to the type of q move the sum by half a step of A (2^-8 bf16, 2^-11
-    half); cut instead, with the row sum of the same cut weights, by a whole step of A + |out| <= 2 A.  The result is rounded by half a step of
-    itself, at most A.  Scores are sums of d products in 32 bits: off by (d + 2) 2^-24 sum |q k| at most, and a weight, relative to the
+    With A = sum_j w_j |v_j|: weights w_j (1 + e_j) in the sum over v and in their own sum give (out + sum w e v) / (1 + sum w e), off by at
+    most (A + |out|) max|e| / (1 - max|e|).  They are rounded to the type of q, e up to half a step (2^-8 bf16, 2^-11 half), or cut, e up to a
+    whole one.  The result is rounded by half a step of itself.  Scores are sums of d products in 32 bits: off by (d + 2) 2^-24 sum |q k| at most, and a weight, relative to the
     others, by twice that.  exp2, sums of weights and the merge of partials in 32 bits: 2^-18 of A is more than they take.
     """
     half_step = torch.finfo(dtype).eps / 2
-    weights = 4 * half_step if cut else half_step
+    weights = half_step * (2 if cut else 1) * (1 + 2.0 ** -6)
     smallest = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -24}[dtype]  # half the step of half's smallest numbers, and weights below them
-    return spread * (weights + half_step + 2 * (d + 2) * 2.0 ** -24 * score[..., None] + 2.0 ** -18) + smallest * (1 + spread)
+    return weights * (spread + out.abs()) + half_step * out.abs() * (1 + half_step * 4) + spread * (2 * (d + 2) * 2.0 ** -24 * score[..., None] + 2.0 ** -18) + smallest * (1 + spread)
 
 
 def assert_within(got, out, spread, tol, what=""):
