@@ -19,26 +19,20 @@ constexpr int kMxBlock = 32;
 constexpr int kMxLeast = 2, kMxMost = 252;  // block bytes
 constexpr int kMxNotFinite = 255;           // in K's
 
-// The block byte for values up to `amax` (finite, not negative): with amax = m 2^e, 1 <= m < 2, the unit is 2^(e - 2) if 4 m <= 6, else 2^(e - 1).
-__device__ __forceinline__ int mx_block_byte(float amax) {
-  const uint32_t bits = __builtin_bit_cast(uint32_t, amax);
+// The block byte for values up to the one with these bits (finite, not negative): with it m 2^e, 1 <= m < 2, the unit is 2^(e - 2) if 4 m <= 6, else 2^(e - 1).
+__device__ __forceinline__ int mx_block_byte(uint32_t bits) {
   return min(max((int)(bits >> 23) - 2 + ((bits & 0x7fffffu) > 0x400000u ? 1 : 0), kMxLeast), kMxMost);
 }
 
-// Eight values as codes, the first in the lowest 4 bits: nearest, halfway to the even code (v_cvt_scalef32_pk_fp4_f32 does
-// both).  The unit is a power of two, so the division by it is exact.
+// Eight values as codes, the first in the lowest 4 bits: divided by the block's unit (exact: of the factor the conversion takes the
+// exponent), nearest, halfway to the even code.
 __device__ __forceinline__ uint32_t mx_codes8(const float (&x)[8], int byte) {
-  const int e = 127 - byte;
+  const float unit = __builtin_bit_cast(float, (uint32_t)byte << 23);
   uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float lo = __builtin_amdgcn_ldexpf(x[2 * i], e), hi = __builtin_amdgcn_ldexpf(x[2 * i + 1], e);
-    r = i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, lo, hi, 1.0f, 0)
-        : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, lo, hi, 1.0f, 1)
-        : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, lo, hi, 1.0f, 2)
-                 : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, lo, hi, 1.0f, 3);
-  }
-  return r;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[0], x[1], unit, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[2], x[3], unit, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[4], x[5], unit, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[6], x[7], unit, 3);
 }
 
 // Codes 2 B and 2 B + 1 of a word as bf16 or, with F16, IEEE half, times 2^(exponent of `scale`): of `scale` the conversion looks at

@@ -12,10 +12,10 @@
 // position * base^(-i / (d/2)) / 2 pi are a product of 64 bits, their fraction is exact, and sine and cosine of what is left, at most an
 // eighth of a turn, are Taylor sums in 64 bits.  (64-bit products issue as fast as 32-bit ones here.)
 //
-// HBM-bound: q, k and v are read once, q and the codes written once.  Sixteen lanes own one token's head: lane j holds elements E j .. E j + E - 1
-// of both halves (E = d / 32), so the rotation pairs are lane-local; a block of 32 dims is 32 / E of them.  The same lanes take K and V of
-// a head, since V that is not finite is noted in K's block bytes.  A group of lanes walks a chunk of the token's heads, and the angles are made once
-// per chunk.
+// HBM-bound: q, k and v are read once, q and the codes written once.  d / 16 lanes own one token's head: lane j holds elements 8 j .. 8 j + 7 of both
+// halves, so the rotation pairs are lane-local, a block of 32 dims is four lanes, and the lanes of a wave take neighbouring heads: whole lines.
+// The same lanes take K and V of a head, since V that is not finite is noted in K's block bytes.  Sines and cosines are made once per
+// workgroup and token, a pair to a thread, and lie in LDS.
 #include <math.h>
 
 #include <type_traits>
@@ -26,8 +26,8 @@
 namespace msgl {
 namespace {
 
-constexpr int kGroupLanes = 16;
 constexpr int kThreads = 256;
+constexpr int kManyTokens = 4;  // of a workgroup, where there are many
 
 template <int D>
 struct Params {
@@ -36,23 +36,23 @@ struct Params {
   uint16_t* q_out;
   unsigned char *codes, *scales;
   int64_t q_stride0, k_stride0, v_stride0, codes_stride, scales_stride, num_slots;
-  uint32_t items, chunks, per_group;  // (token, chunk of heads)
-  int32_t n_q, n_kv;
+  int32_t n_tokens, n_q, n_kv;
+  uint32_t chunks;  // workgroups to a token's heads
   double eps;
   double turns[D / 2];  // base^(-i / (d/2)) / 2 pi
 };
 
-__device__ __forceinline__ double dpp_sum16(double v) {
-  auto add = [&](auto control) {
-    constexpr int C = decltype(control)::value;
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint64_t o = (uint64_t)(uint32_t)dpp<C>((int)(u >> 32)) << 32 | (uint32_t)dpp<C>((int)(uint32_t)u);
-    v += __builtin_bit_cast(double, o);
-  };
-  add(std::integral_constant<int, 0xB1>{});
-  add(std::integral_constant<int, 0x4E>{});
-  add(std::integral_constant<int, 0x141>{});
-  add(std::integral_constant<int, 0x140>{});
+template <int C>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)dpp<C>((int)(u >> 32)) << 32 | (uint32_t)dpp<C>((int)(uint32_t)u));
+}
+template <int LANES>  // 8 or 16
+__device__ __forceinline__ double sum_over(double v) {
+  v += dpp64<0xB1>(v);
+  v += dpp64<0x4E>(v);
+  v += dpp64<0x141>(v);
+  if constexpr (LANES == 16) v += dpp64<0x140>(v);
   return v;
 }
 
@@ -89,121 +89,133 @@ __device__ __forceinline__ void sine_cosine(double turns, float* sine, float* co
   *cosine = (n == 1 || n == 2) ? -b : b;
 }
 
-template <int E>
-struct Half;  // E bf16 values as one load
-template <>
-struct Half<4> { typedef u32x2_t type; };
-template <>
-struct Half<8> { typedef u32x4_t type; };
+// 16 values of a lane: 8 of the lower half of a head and 8 of the upper
+struct Row {
+  u32x4_t lo, hi;
+};
+__device__ __forceinline__ void values_of(const Row& r, float (&x)[16]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t l = r.lo[e >> 1], h = r.hi[e >> 1];
+    x[e] = __builtin_bit_cast(float, (e & 1) ? l & 0xffff0000u : l << 16);
+    x[8 + e] = __builtin_bit_cast(float, (e & 1) ? h & 0xffff0000u : h << 16);
+  }
+}
+// The bits of the largest of a half's values; what is not finite is above all others
+__device__ __forceinline__ uint32_t largest(const float (&x)[16], int half) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, x[8 * half + e]) & 0x7fffffffu);
+  return top;
+}
 
-template <int D>
+template <int D, int TOKENS>
 __global__ __launch_bounds__(kThreads) void norm_rope_store_mxfp4_kernel(Params<D> p) {
-  constexpr int E = D / 32, kBlockLanes = kMxBlock / E;
-  using V = typename Half<E>::type;
-  const int j = threadIdx.x & (kGroupLanes - 1);
-  const uint32_t item = blockIdx.x * (kThreads / kGroupLanes) + threadIdx.x / kGroupLanes;
-  if (item >= p.items) return;  // whole groups leave together, and nothing crosses groups
-  const uint32_t token = item / p.chunks, chunk = item - token * p.chunks;
-  const int n_heads = p.n_q + p.n_kv, h_begin = chunk * p.per_group, h_end = min(h_begin + (int)p.per_group, n_heads);
-  const int off = j * E;
-  struct Row {
-    V lo, hi;
+  constexpr int kLanes = D / 16, kGroups = kThreads / kLanes / TOKENS;  // groups of lanes to a token
+  __shared__ __attribute__((aligned(16))) float2 angles[TOKENS][D / 2];
+  const uint32_t block = blockIdx.x / p.chunks, chunk = blockIdx.x - block * p.chunks;
+  const int group = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
+  const int first = (int)block * TOKENS, sub = group / kGroups;
+  const int token = min(first + sub, p.n_tokens - 1);  // of the last again, where there are no more: nothing is stored
+  const bool live = first + sub < p.n_tokens;
+  const int off = j * 8, units = p.n_q + p.n_kv;
+  const uint16_t *q = p.q + token * p.q_stride0 + off, *k = p.k + token * p.k_stride0 + off, *v = p.v + token * p.v_stride0 + off;
+  auto load = [](const uint16_t* row) { return Row{ld_global_b128(row), ld_global_b128(row + D / 2)}; };
+  // a unit: a q head, or K and V of a kv head.  The lanes of a wave have neighbouring units, and the next ones' rows are under way
+  struct Unit {
+    Row a, b;
   };
-  auto fetch = [&](const uint16_t* row) { return Row{*reinterpret_cast<const V*>(row + off), *reinterpret_cast<const V*>(row + D / 2 + off)}; };
-  auto value = [](const V& r, int e) {
-    const uint32_t w = r[e >> 1];
-    return __builtin_bit_cast(float, (e & 1) ? w & 0xffff0000u : w << 16);
+  auto fetch = [&](int u) {
+    Unit x{};
+    if (u < p.n_q) {
+      x.a = load(q + u * D);
+    } else if (u < units) {
+      x.a = load(k + (u - p.n_q) * D);
+      x.b = load(v + (u - p.n_q) * D);
+    }
+    return x;
   };
-  const double position = (double)p.positions[token];
+  const int step = kGroups * (int)p.chunks;
+  int u = (int)chunk * kGroups + group % kGroups;
+  Unit next = fetch(u);
   const int64_t slot = p.out_loc[token];
-  float cs[E], sn[E];
+  float q_weight[16], k_weight[16];
+  values_of(load(p.q_weight + off), q_weight);
+  values_of(load(p.k_weight + off), k_weight);
 #pragma unroll
-  for (int e = 0; e < E; ++e) sine_cosine(position * p.turns[off + e], &sn[e], &cs[e]);
+  for (int at = threadIdx.x; at < TOKENS * (D / 2); at += kThreads) {
+    const int t = at / (D / 2), pair = at % (D / 2);
+    float2 a;
+    sine_cosine((double)p.positions[min(first + t, p.n_tokens - 1)] * p.turns[pair], &a.y, &a.x);
+    angles[t][pair] = a;
+  }
+  __syncthreads();
+  float cs[8], sn[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    cs[e] = angles[sub][off + e].x;
+    sn[e] = angles[sub][off + e].y;
+  }
 
-  // x: in order the E values of the lower half and those of the upper
-  auto load = [&](const uint16_t* row, float (&x)[2 * E]) {
-    const Row r = fetch(row);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] = value(r.lo, e);
-      x[E + e] = value(r.hi, e);
-    }
-  };
-  auto rotate = [&](float (&x)[2 * E], const uint16_t* weight) {
+  auto rotate = [&](float (&x)[16], const float (&w)[16]) {
 #pragma clang fp contract(off)
-    float w[2 * E];
-    load(weight, w);
-    double ss = 0.0;
+    double lo = 0.0, hi = 0.0;
 #pragma unroll
-    for (int e = 0; e < 2 * E; ++e) ss = fma((double)x[e], (double)x[e], ss);
-    ss = dpp_sum16(ss);
-    const float factor = (float)reciprocal_root(ss * (1.0 / D) + p.eps);
+    for (int e = 0; e < 8; ++e) {
+      lo = fma((double)x[e], (double)x[e], lo);
+      hi = fma((double)x[8 + e], (double)x[8 + e], hi);
+    }
+    const float factor = (float)reciprocal_root(sum_over<kLanes>(lo + hi) * (1.0 / D) + p.eps);
 #pragma unroll
-    for (int e = 0; e < 2 * E; ++e) x[e] = w[e] * (x[e] * factor);
+    for (int e = 0; e < 16; ++e) x[e] = w[e] * (x[e] * factor);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float a = x[e], b = x[E + e];
+    for (int e = 0; e < 8; ++e) {
+      const float a = x[e], b = x[8 + e];
       x[e] = a * cs[e] - b * sn[e];
-      x[E + e] = a * sn[e] + b * cs[e];
+      x[8 + e] = a * sn[e] + b * cs[e];
     }
   };
-  // The codes of a row at `codes` and its block bytes at `scales`; poison: the row counts as zeros, `mark`: and its block bytes say so
-  auto store = [&](const float (&in)[2 * E], unsigned char* codes, unsigned char* scales, bool poison, bool mark) {
+  for (; u < units; u += step) {
+    const Unit now = next;
+    next = fetch(u + step);
+    float x[16];
+    values_of(now.a, x);
+    if (u < p.n_q) {
+      rotate(x, q_weight);
+      if (!live) continue;
+      uint16_t* dst = p.q_out + ((int64_t)token * p.n_q + u) * D + off;
+      u32x4_t lo, hi;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float x[8], amax = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        x[e] = poison ? 0.f : in[half * E + e];
-        amax = fmaxf(amax, fabsf(x[e]));
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+        hi[e] = pack_bf16x2(x[8 + 2 * e], x[8 + 2 * e + 1]);
       }
-      amax = fmaxf(amax, dpp<0xB1>(amax));
-      amax = fmaxf(amax, dpp<0x4E>(amax));
-      if constexpr (kBlockLanes == 8) amax = fmaxf(amax, dpp<0x141>(amax));
-      const int byte = mx_block_byte(amax);
-      const uint32_t word = mx_codes8(x, byte);
-      unsigned char* to = codes + half * (D / 4) + j * (E / 2);
-      if constexpr (E == 8) *reinterpret_cast<uint32_t*>(to) = word;
-      else *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
-      if (j % kBlockLanes == 0) scales[half * (D / 64) + j / kBlockLanes] = (unsigned char)(poison && mark ? kMxNotFinite : byte);
-    }
-  };
-  auto any_not_finite = [&](const float (&x)[2 * E]) {
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 2 * E; ++e) bad |= (__builtin_bit_cast(uint32_t, x[e]) & 0x7f800000u) == 0x7f800000u;
-    return bad;
-  };
-
-  for (int h = h_begin; h < h_end; ++h) {
-    if (h < p.n_q) {
-      float x[2 * E];
-      load(p.q + token * p.q_stride0 + h * D, x);
-      rotate(x, p.q_weight);
-      uint16_t* dst = p.q_out + ((int64_t)token * p.n_q + h) * D + off;
-      V lo, hi;
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        lo[e >> 1] = pack_bf16x2(x[e], x[e + 1]);
-        hi[e >> 1] = pack_bf16x2(x[E + e], x[E + e + 1]);
-      }
-      *reinterpret_cast<V*>(dst) = lo;
-      *reinterpret_cast<V*>(dst + D / 2) = hi;
+      st_global_b128(dst, lo);
+      st_global_b128(dst + D / 2, hi);
     } else {
-      const int kvh = h - p.n_q;
-      float k[2 * E], v[2 * E];
-      load(p.k + token * p.k_stride0 + kvh * D, k);
-      load(p.v + token * p.v_stride0 + kvh * D, v);
-      rotate(k, p.k_weight);
-      const uint64_t group = 0xffffull << (lane_id() & ~(kGroupLanes - 1));
-      const bool poison = (__ballot(any_not_finite(k) || any_not_finite(v)) & group) != 0;
-      if ((uint64_t)slot >= (uint64_t)p.num_slots) continue;
-      unsigned char* codes = p.codes + slot * p.codes_stride + kvh * D;
-      unsigned char* scales = p.scales + slot * p.scales_stride + kvh * (D / 16);
-      store(k, codes, scales, poison, true);
-      store(v, codes + D / 2, scales + D / 32, poison, false);
+      rotate(x, k_weight);
+      float y[16];
+      values_of(now.b, y);
+      uint32_t top[4] = {largest(x, 0), largest(x, 1), largest(y, 0), largest(y, 1)};
+      const uint64_t mine = ((1ull << kLanes) - 1) << (lane_id() & ~(kLanes - 1));
+      const bool poison = (__ballot(max(max(top[0], top[1]), max(top[2], top[3])) >= 0x7f800000u) & mine) != 0;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {  // the block's
+        top[h] = max(top[h], (uint32_t)dpp<0xB1>((int)top[h]));
+        top[h] = max(top[h], (uint32_t)dpp<0x4E>((int)top[h]));
+      }
+      if (!live || (uint64_t)slot >= (uint64_t)p.num_slots) continue;
+      unsigned char* codes = p.codes + slot * p.codes_stride + (u - p.n_q) * D;
+      unsigned char* scales = p.scales + slot * p.scales_stride + (u - p.n_q) * (D / 16);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {  // K's halves, V's halves
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = poison ? 0.f : h < 2 ? x[8 * h + e] : y[8 * (h - 2) + e];
+        const int byte = mx_block_byte(poison ? 0u : top[h]);
+        *reinterpret_cast<uint32_t*>(codes + h * (D / 4) + j * 4) = mx_codes8(z, byte);
+        if ((j & 3) == 0) scales[h * (D / 64) + (j >> 2)] = (unsigned char)(poison && h < 2 ? kMxNotFinite : byte);
+      }
     }
   }
 }
@@ -234,14 +246,14 @@ int launch(const Mxfp4NormRopeArgs& a, hipStream_t stream) {
   const long double step = powl((long double)a.rope_base, -2.0L / D);
   long double turn = 0.159154943091895335768883763372514362L;  // 1 / 2 pi
   for (int i = 0; i < D / 2; ++i, turn *= step) p.turns[i] = (double)turn;
-  // one head per group until its workgroups fill the chip twice over: few tokens are the chain of one group's loads
-  const int64_t n_heads = a.n_q + a.pool.n_kv;
-  p.per_group = a.n_tokens * n_heads <= 512 * (kThreads / kGroupLanes) ? 1 : 8;
-  p.chunks = (uint32_t)((n_heads + p.per_group - 1) / p.per_group);
-  const int64_t items = a.n_tokens * p.chunks, per_block = kThreads / kGroupLanes;
-  if (items >= (int64_t)1 << 31) return MSGL_ERR_SHAPE;
-  p.items = (uint32_t)items;
-  return launch_kernel(norm_rope_store_mxfp4_kernel<D>, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(kThreads), stream, p);
+  // A workgroup has four tokens where that fills the chip twice over: it makes their angles with all its threads.  Else a token or a part of its heads
+  const bool many = a.n_tokens >= 2 * kManyTokens * (int64_t)device_cus();
+  constexpr int kUnits = kThreads / (D / 16);
+  p.n_tokens = (int32_t)a.n_tokens;
+  p.chunks = many ? 1u : (uint32_t)((a.n_q + a.pool.n_kv + kUnits - 1) / kUnits);
+  const int64_t blocks = many ? (a.n_tokens + kManyTokens - 1) / kManyTokens : a.n_tokens * p.chunks;
+  if (a.n_tokens > 0x7fffffffLL || blocks > 0x7fffffffLL) return MSGL_ERR_SHAPE;
+  return launch_kernel(many ? norm_rope_store_mxfp4_kernel<D, kManyTokens> : norm_rope_store_mxfp4_kernel<D, 1>, dim3((unsigned)blocks), dim3(kThreads), stream, p);
 }
 
 }  // namespace

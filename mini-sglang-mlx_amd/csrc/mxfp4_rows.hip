@@ -13,7 +13,6 @@ __device__ __forceinline__ float value16(uint32_t w, int half, bool f16) {
   const uint32_t h = half ? w >> 16 : w & 0xffffu;
   return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __builtin_bit_cast(float, h << 16);
 }
-__device__ __forceinline__ bool not_finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) == 0x7f800000u; }
 // Or over the 16 lanes' four groups of four, whose lanes agree
 __device__ __forceinline__ uint32_t or_of_blocks(uint32_t v) {
   v |= (uint32_t)dpp<0x124>((int)v);  // the lane 4 below, with rotation
@@ -40,25 +39,24 @@ __global__ __launch_bounds__(kThreads) void store_mxfp4_kernel(StoreParams p) {
   const uint16_t* src = (of_v ? p.v + row * p.v_stride0 : p.k + row * p.k_stride0) + head * D + j * 8;
   const int64_t slot = p.indices[row];
   const u32x4_t raw = ld_global_b128(src);
-  float x[8], amax = 0.f;
-  bool bad = false;
+  float x[8];
+  uint32_t top = 0;  // the largest value's bits, with what is not finite above all others
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     x[e] = value16(raw[e >> 1], e & 1, F16);
-    bad |= not_finite(x[e]);
-    amax = fmaxf(amax, fabsf(x[e]));
+    top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
   }
   // one lane's is everybody's of the (row, kv head)
   const uint64_t of_item = kLanes == 64 ? ~0ull : ((1ull << (kLanes & 63)) - 1) << (lane_id() & ~(kLanes - 1) & 63);
-  const bool poison = (__ballot(bad) & of_item) != 0;
-  amax = fmaxf(amax, dpp<0xB1>(amax));
-  amax = fmaxf(amax, dpp<0x4E>(amax));
+  const bool poison = (__ballot(top >= 0x7f800000u) & of_item) != 0;
+  top = max(top, (uint32_t)dpp<0xB1>((int)top));
+  top = max(top, (uint32_t)dpp<0x4E>((int)top));
   if (poison) {
-    amax = 0.f;
+    top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 0.f;
   }
-  const int byte = mx_block_byte(amax);
+  const int byte = mx_block_byte(top);
   const uint32_t codes = mx_codes8(x, byte);
   const uint32_t scales = or_of_blocks((uint32_t)(poison && !of_v ? kMxNotFinite : byte) << (8 * ((lane >> 2) & 3)));
   if (!live || (uint64_t)slot >= (uint64_t)p.num_slots) return;
