@@ -291,7 +291,7 @@ struct Mxfp4AttentionArgs {
 };
 // most columns (queries of a request times q heads of a kv head) of a launch
 int64_t mxfp4_max_columns(int64_t head_dim);
-size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t total_kv, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend);
+size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend);
 int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream);
 
 // A launch without the triple brackets' detour (they put the configuration away and fetch it again, 0.2 us of host time).

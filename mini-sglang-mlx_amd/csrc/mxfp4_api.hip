@@ -124,7 +124,7 @@ int msgl_qk_norm_rope_store_mxfp4(const void* q, const void* k, const void* v, i
 
 size_t msgl_paged_decode_mxfp4_workspace_bytes(int64_t batch, int64_t total_kv, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim) {
   if (batch <= 0 || total_kv < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0) return 0;
-  return msgl::mxfp4_attention_workspace_bytes(batch, total_kv, num_q_heads, num_kv_heads, head_dim, 1);
+  return msgl::mxfp4_attention_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, 1);
 }
 
 int msgl_paged_decode_attention_mxfp4(const void* q, const void* kv_codes, const void* kv_scales, const int32_t* kv_indptr,
@@ -144,7 +144,7 @@ int msgl_paged_decode_attention_mxfp4(const void* q, const void* kv_codes, const
   if (const int rc = check_pool(a.pool)) return rc;
   if (!aligned16(q) || !aligned16(out)) return MSGL_ERR_ALIGNMENT;
   if (!workspace || !aligned16(workspace) ||
-      workspace_bytes < msgl::mxfp4_attention_workspace_bytes(batch, total_kv, num_q_heads, num_kv_heads, head_dim, 1))
+      workspace_bytes < msgl::mxfp4_attention_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, 1))
     return MSGL_ERR_WORKSPACE;
   a.q = q;
   a.kv_indptr = kv_indptr;
@@ -164,7 +164,7 @@ size_t msgl_paged_prefill_mxfp4_workspace_bytes(int64_t batch, int64_t total_q, 
                                                 int64_t head_dim, int64_t max_len_extend) {
   if (batch <= 0 || total_q < 0 || total_kv < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || max_len_extend <= 0) return 0;
   if (reads_pool(num_q_heads, num_kv_heads, head_dim, max_len_extend))
-    return msgl::mxfp4_attention_workspace_bytes(batch, total_kv, num_q_heads, num_kv_heads, head_dim, max_len_extend);
+    return msgl::mxfp4_attention_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_len_extend);
   return std::max<size_t>(256, unpacked(total_kv, num_kv_heads, head_dim).rest +
                                    msgl_paged_prefill_workspace_bytes(batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, max_len_extend));
 }

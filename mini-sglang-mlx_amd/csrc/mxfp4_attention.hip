@@ -1,456 +1,402 @@
-// Attention over a K/V pool in 4 bits (mxfp4.h) for short query blocks: decode, speculative verify, drafts.
+// Attention over a K/V pool in 4 bits for decode and short query blocks: mxfp4_tiles.h, one workgroup to a share of a request's keys for one to eight kv heads.
 //
-//   out[c] = sum_j w_cj v_j / sum_j w_cj,  w_cj = exp(sm_scale q_c . k_j - m_c),  over the keys j that column c sees
+// Each request's visible keys are cut into equal shares, as many in all as there are workgroups that the card holds at once, one to a CU; the waves of a
+// workgroup take a head each, or cut a head's share again and meet in LDS; and of a request that several shares hold the workgroup that counts last puts
+// the partials together.  One launch, and nobody waits for anybody: a merge in a launch of its own took 8 us of small calls and 12 of 32 requests of 32 columns,
+// and equal parts of the stream of all keys, which begin and end inside requests, as long as whole shares or longer (64 requests of 8 K keys 109
+// us against 107, 8 of 4 K 18.7 against 16.3).  Partials and counts travel at agent scope; a count word carries the launch's number
+// (launch_number.h), so the workspace needs no clearing, and is left as of a launch that never happened, so a replay counts anew.
 //
-// Bound by memory: a key of a kv head is D + D / 16 bytes, of its request 4 more, and everything a column needs is computed from one pass
-// over them with the running maximum m and sum.  The visible keys of all requests are one stream, cut into equal segments
-// (splitkv_stream.h); a wave takes a segment for one kv head, and partials of requests that several segments share are merged by a
-// second launch.
-//
-// One wave, 32 keys:
-//   S^T = K Q^T    mfma 16x16x32, keys on M.  Lane (r, g) of the operand holds 32 dims of its key, block 4 h + g of half h: 16 bytes of codes and one
-//                  block byte.  Four products take 8 dims of every block each, which is an order of the contraction like any other, and Q is
-//                  read in the same.
-//   O^T += V^T P^T mfma 16x16x32, dims on M.  Lane (r, g) reads dims 8 r .. 8 r + 7 of half h, one word, of each of the 8 keys of group g, and turns the 8 x 8 values
-//                  over after the conversion.  Row 4 a + i of product u of S^T is key 8 a + of_group(4 u + i), so the
-//                  weights of group g's keys are the ones that its lanes hold.
-// The conversion multiplies by the block's factor on the way (one instruction for two values), so codes cost what 16-bit values would.
-// Weights are rounded to the type of q for the second product (half a step, 2^-8 and 2^-11 of a weight, as the 16-bit pool's
-// kernels do); scores, sums and accumulators have 32 bits, and so do the partials.
-#include <type_traits>
+// Bound by memory: 16 requests of 32-128 K keys of 8 heads of 128, 6.0 TB/s; 64 of 512-8 K 5.3.
+#include <cmath>
+#include <utility>
 
-#include "mxfp4.h"
-#include "prefill_tile_common.h"
-#include "splitkv_stream.h"
+#include "agent_scope.h"
+#include "launch_number.h"
+#include "mxfp4_tiles.h"
 
 namespace msgl {
 namespace {
 
-struct MxParams : SplitKvParams {
-  int32_t negate;  // scale_log2e is positive: with a scale below zero (-1) the scores of -q count, with none (1) those of zeros
+struct ShareParams : MxParams {
+  unsigned long long* counts;     // [batch][head_groups][kCountWords]: shares done
+  unsigned long long nonce;       // launch_number.h
+  int32_t shares;                 // as many as there may be ..
+  float min_len;                  // .. if that makes none shorter
+  int32_t wave_shift;             // log2 of the waves on a head's share
 };
 
+// A share's place: number `share` of the `n_shares` of request b, number `item` of the launch
+struct MxShare {
+  ReqInfo r;
+  int b, share, n_shares, item;
+};
+// How requests are cut: the shortest length of a share, min_len at least, with which there are no more shares than fit on the card at once.  It is between
+// total / shares and what is enough when every request loses a whole share to its end, and the wave that wants to know looks for it there: 64 requests at a
+// time, which stay in registers up to kCached of them.  (Beyond those, and where even a share to a request is too many, the outer end is taken.)
+constexpr int kCached = 256;
+constexpr float kOneShare = 0x1p31f;  // keys, no request has more
+// (The quotient of floats may take an exact one a share too far, never two; `max_shares` of the launch has room for a share more of every request that has keys.)
+__device__ __forceinline__ int shares_of(int visible, float per_len) { return (int)ceilf((float)visible * per_len); }
+
+// All lanes must call; false past the last share.
+__device__ __forceinline__ bool find_mx_share(const ShareParams& p, int item, MxShare* x) {
+  const int lane = lane_id();
+  auto visible_of = [&](const ReqInfo& r, int b0) { return b0 + lane < p.batch ? max(r.hi - r.lo, 0) : 0; };
+  auto request_at = [&](int b0) { return request_info(p, min(b0 + lane, p.batch - 1)); };
+  const ReqInfo first64 = request_at(0);
+  int visible[kCached / kWave];
+  visible[0] = visible_of(first64, 0);
+  int total = wave_sum(visible[0]), some = __popcll(__ballot(visible[0] > 0));
+#pragma unroll
+  for (int c = 1; c < kCached / kWave; ++c) {
+    visible[c] = 0;
+    if (c * kWave >= p.batch) continue;
+    visible[c] = visible_of(request_at(c * kWave), c * kWave);
+    total += wave_sum(visible[c]);
+    some += __popcll(__ballot(visible[c] > 0));
+  }
+  for (int b0 = kCached; b0 < p.batch; b0 += kWave) {
+    const int n = visible_of(request_at(b0), b0);
+    total += wave_sum(n);
+    some += __popcll(__ballot(n > 0));
+  }
+  auto fit = [&](float len) {
+    const float per_len = __builtin_amdgcn_rcpf(len);
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < kCached / kWave; ++c)
+      if (c * kWave < p.batch) n += shares_of(visible[c], per_len);
+    return wave_sum(n) <= p.shares;
+  };
+  float len = fmaxf((float)total * __builtin_amdgcn_rcpf((float)p.shares), p.min_len);  // from here ..
+  float most = some < p.shares ? fmaxf((float)total * __builtin_amdgcn_rcpf((float)(p.shares - some)), p.min_len) : kOneShare;  // .. to here
+  if (some >= p.shares || p.batch > kCached) {
+    len = most;
+  } else if (!fit(len)) {
+    while (most > len * (1.f + 1.f / 32)) {
+      const float mid = 0.5f * (len + most);
+      if (fit(mid)) most = mid;
+      else len = mid;
+    }
+    len = most;
+  }
+  const float per_len = __builtin_amdgcn_rcpf(len);
+  int base = 0;
+  auto here = [&](int n_visible, int b0, auto&& request) {
+    // a request without visible keys has one empty share: its rows are zero
+    const int n = b0 + lane < p.batch ? max(shares_of(n_visible, per_len), 1) : 0;
+    const int incl = wave_inclusive_scan(n), sum = __builtin_amdgcn_readlane(incl, kWave - 1), first = base + incl - n;
+    base += sum;
+    if (item >= base) return false;
+    const int src = __builtin_amdgcn_readfirstlane(__ffsll((long long)__ballot(item >= first && item < first + n)) - 1);
+    x->r = request(src);
+    x->b = b0 + src;
+    x->share = item - __builtin_amdgcn_readlane(first, src);
+    x->n_shares = __builtin_amdgcn_readlane(n, src);
+    x->item = item;
+    return true;
+  };
+  if (here(visible[0], 0, [&](int src) {
+        ReqInfo r;
+        r.kv_start = __builtin_amdgcn_readlane(first64.kv_start, src);
+        r.kv_len = __builtin_amdgcn_readlane(first64.kv_len, src);
+        r.q_start = __builtin_amdgcn_readlane(first64.q_start, src);
+        r.q_len = __builtin_amdgcn_readlane(first64.q_len, src);
+        r.prefix = __builtin_amdgcn_readlane(first64.prefix, src);
+        r.lo = __builtin_amdgcn_readlane(first64.lo, src);
+        r.hi = __builtin_amdgcn_readlane(first64.hi, src);
+        r.rows = __builtin_amdgcn_readlane(first64.rows, src);
+        return r;
+      }))
+    return true;
+#pragma unroll
+  for (int c = 1; c < kCached / kWave; ++c) {
+    if (c * kWave >= p.batch) return false;
+    if (here(visible[c], c * kWave, [&](int src) { return request_info(p, c * kWave + src); })) return true;
+  }
+  for (int b0 = kCached; b0 < p.batch; b0 += kWave)
+    if (here(visible_of(request_at(b0), b0), b0, [&](int src) { return request_info(p, b0 + src); })) return true;
+  return false;
+}
+
+// The LDS of a workgroup: a wave's stages, and in their place, when its keys are done, its accumulators.
 template <int D, int NCT>
-struct MxColumns {
-  u32x4_t q[NCT][D / 32];      // [4 h + c]: dims 128 h + 32 g + 8 c ..
-  int lo[NCT], hi[NCT];        // first and last visible key of this lane's column in each tile of 16
-  int all_lo, all_hi;          // keys inside are visible to every column
-  float m[NCT], l[NCT];        // what the weights are relative to (base 2; 0 before the first key); this lane's part of their sum
-  float top[NCT];              // m, or -infinity before the first key
-  f32x4_t o[NCT][D / 128][8];  // [h][n][i]: dim 128 h + 8 (4 g + i) + n
+struct WavePart {
+  static constexpr int kBlock = 16 * NCT * 8 + 8;  // floats of 8 dims: [col][8], padded
+  float o[D / 8][kBlock];
+};
+template <int D, int NCT, int NW>
+struct MxLds {
+  static constexpr int kWaveBytes = (std::max(sizeof(WaveLds<D>), sizeof(WavePart<D, NCT>)) + 255) / 256 * 256;
+  unsigned char wave[NW][kWaveBytes];
+  float2 state[NW][16 * NCT];  // (reference, sum) of a wave's columns
+  int last;
 };
 
-template <int D>
-struct MxTile {  // 32 keys as they lie in the pool
-  u32x4_t k[D / 128][2];
-  uint32_t k_byte[D / 128][2];
-  uint32_t v[D / 128][8], v_byte[D / 128][8];
-};
-
-// The factor of a block as the conversion wants it.  Half reaches 65504 = 2^16 (1 - 2^-11) while a block that holds that much has the unit 2^14 and codes up to
-// 6: K and V come in at half their size there, and scores and results are doubled.
-template <bool F16, bool IS_K>
-__device__ __forceinline__ float block_factor(uint32_t byte) {
-  if constexpr (!F16) return mx_scale(byte);
-  else if constexpr (IS_K) return mx_scale(byte == kMxNotFinite ? byte : byte - 1);
-  else return mx_scale(byte - 1);
+template <typename F, int... I>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
 }
-template <bool F16>
-constexpr float kBack = F16 ? 2.f : 1.f;
 
-template <int D, int NCT, bool F16>
-__device__ __forceinline__ void start_mx_columns(const MxParams& p, const ReqInfo& r, int kvh, int t_end, MxColumns<D, NCT>& c_) {
-  const int t16 = lane_id() & 15, g = lane_id() >> 4;
-  const int ncols = r.q_len * p.group;
-  int all_lo = 0, all_hi = 0x7fffffff;
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    const int col = ct * 16 + t16;
-    const bool valid = col < ncols;
-    const int qi = valid ? query_of(p, col) : 0;
-    const int hh = valid ? col - qi * p.group : 0;
-    const uint16_t* qrow = p.q + (int64_t)(r.q_start + qi) * p.q_stride0 + (kvh * p.group + hh) * D + g * 32;
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      c_.q[ct][s] = u32x4_t{0u, 0u, 0u, 0u};
-      if (valid) c_.q[ct][s] = ld_global_b128(qrow + (s >> 2) * 128 + (s & 3) * 8);
-      if (p.negate != 0) c_.q[ct][s] = p.negate < 0 ? c_.q[ct][s] ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
-    }
-    const int qpos = r.prefix + qi;
-    int lo = (p.window > 0) ? qpos - p.window + 1 : 0;
-    int hi = min(p.is_cross ? r.kv_len - 1 : min(qpos, r.kv_len - 1), t_end - 1);
-    if (valid) {
-      all_lo = max(all_lo, lo);
-      all_hi = min(all_hi, hi);
-    } else {
-      lo = 1;
-      hi = 0;
-    }
-    c_.lo[ct] = lo;
-    c_.hi[ct] = hi;
+// A wave's place in its workgroup: waves on a head, which head, which of its waves
+struct MxWave {
+  int waves, sub, sw, threads, me;  // threads on a head, this one's number
+  __device__ __forceinline__ explicit MxWave(const ShareParams& p) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    waves = 1 << p.wave_shift;
+    sub = wave >> p.wave_shift;
+    sw = wave & (waves - 1);
+    threads = 64 << p.wave_shift;
+    me = (int)threadIdx.x - sub * threads;
   }
-  c_.all_lo = __builtin_amdgcn_readfirstlane(row_max16(all_lo));
-  c_.all_hi = __builtin_amdgcn_readfirstlane(~row_max16(~all_hi));
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    c_.m[ct] = 0.f;
-    c_.top[ct] = kNegInf;
-    c_.l[ct] = 0.f;
-#pragma unroll
-    for (int h = 0; h < D / 128; ++h)
-#pragma unroll
-      for (int n = 0; n < 8; ++n) c_.o[ct][h][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+};
+// A wave's keys of a share
+struct MxRange {
+  int begin, end;
+  __device__ __forceinline__ MxRange(const ShareParams& p, const MxShare& x, const MxWave& w) {
+    const int per = ((x.r.hi - x.r.lo + x.n_shares - 1) / x.n_shares + 31) & ~31;
+    const int s_begin = min(x.r.lo + x.share * per, x.r.hi), s_end = min(s_begin + per, x.r.hi);
+    const int per_wave = (((per + w.waves - 1) >> p.wave_shift) + 31) & ~31;
+    begin = min(s_begin + w.sw * per_wave, s_end);
+    end = min(begin + per_wave, s_end);
   }
-}
-
-// Where the 32 keys of a tile lie in a wave's stage of LDS, and who takes them to registers.  A load moves 1 KiB: whole slots of a head (8 at
-// head_dim 128, 4 at 256), 16 bytes a lane, which come to lie one behind the other; the 16-byte pieces of a row are exchanged among
-// themselves so that the 16 lanes of a read find theirs in different banks.
-//   row(key), piece c at place c ^ turn(key) of its row
-// Keys of a lane group's 8, in the order n = 4 u + i in which S^T has them (row 4 a + i of product u): of_group(n).
-template <int D>
-struct Place;
-template <>
-struct Place<128> {
-  static constexpr int kLoads = 4, kScaleLoads = 1, kLanes = 8;  // lanes to a row in a load
-  static __device__ __forceinline__ constexpr int of_group(int n) { return (n & 1) + 4 * ((n >> 1) & 1) + 2 * (n >> 2); }
-  // load u, lanes 8 j ..: key 4 j + u
-  static __device__ __forceinline__ int key(int u, int j) { return 4 * j + u; }
-  static __device__ __forceinline__ constexpr int row(int key) { return 8 * (key & 3) + (key >> 2); }
-  static __device__ __forceinline__ constexpr int turn(int key) { return ((key >> 3) & 3) | ((key & 1) << 2); }
-  // What a lane reads, as the sum of its own part and one of the instruction: lane (4 a + i, g) piece g of key 8 a + of_group(4 u + i), ...
-  static __device__ __forceinline__ int k_lane(int a, int i, int g) { return (8 * (i & 1) + 2 * a + (i >> 1)) * 128 + ((g ^ a) + 4 * (i & 1)) * 16; }
-  static __device__ __forceinline__ int k_lane_h(int a, int i, int g) { return k_lane(a, i, g); }
-  static __device__ __forceinline__ constexpr int k_of(int u) { return 16 * 128 * u; }
-  static __device__ __forceinline__ int k_byte(int a, int i, int g) { return (8 * a + of_group(i)) * 8 + g; }
-  // ... and word 4 a + i of V of key 8 g + of_group(n)
-  static __device__ __forceinline__ int v_lane(int a, int i, int g) { return 2 * g * 128 + (a ^ g) * 16 + i * 4; }
-  static __device__ __forceinline__ constexpr int v_of(int n, int) { return (8 * ((n & 1) + 2 * (n >> 2)) + ((n >> 1) & 1)) * 128 + (n & 1 ? 0 : 64); }
-};
-template <>
-struct Place<256> {
-  static constexpr int kLoads = 8, kScaleLoads = 2, kLanes = 16;
-  static __device__ __forceinline__ constexpr int of_group(int n) { return n; }
-  static __device__ __forceinline__ int key(int u, int j) { return 8 * j + u; }
-  static __device__ __forceinline__ constexpr int row(int key) { return 4 * (key & 7) + (key >> 3); }
-  static __device__ __forceinline__ constexpr int turn(int key) { return (key >> 3) | ((key & 3) << 2); }
-  static __device__ __forceinline__ int k_lane(int a, int i, int g) { return (4 * i + a) * 256 + (4 * i + (g ^ a)) * 16; }
-  static __device__ __forceinline__ int k_lane_h(int a, int i, int g) { return (4 * i + a) * 256 + (4 * (i ^ 1) + (g ^ a)) * 16; }
-  static __device__ __forceinline__ constexpr int k_of(int u) { return 16 * 256 * u; }
-  static __device__ __forceinline__ int k_byte(int a, int i, int g) { return (8 * a + i) * 16 + g; }
-  static __device__ __forceinline__ int v_lane(int a, int i, int g) { return g * 256 + (a ^ g) * 16 + i * 4; }
-  static __device__ __forceinline__ constexpr int v_of(int n, int h) { return 4 * n * 256 + ((2 + h) ^ (n & 3)) * 64; }
 };
 
-// sum + both weights of a pair
-template <bool F16>
-__device__ __forceinline__ float add_weights(uint32_t pair, float sum) {
-  if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pair), f16x2_t{(_Float16)1.f, (_Float16)1.f}, sum, false);
-  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), kOnes, sum, false);
+// Four dims of a column of the result
+template <int D, bool F16>
+__device__ __forceinline__ void leave_quad(const ShareParams& p, const ReqInfo& r, int kvh, int col, int d4, f32x4_t o) {
+  const int qi = query_of(p, col);
+  uint16_t* dst = p.out + ((int64_t)(r.q_start + qi) * p.n_q + kvh * p.group + (col - qi * p.group)) * D + d4;
+  *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{pack_16x2<F16>(o[0], o[1]), pack_16x2<F16>(o[2], o[3])};
 }
 
-// Keys tb .. tb + 31 for the columns in `c_`
-template <int D, int NCT, bool F16>
-__device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const MxTile<D>& t, int tb, MxColumns<D, NCT>& c_) {
-  const int g = lane_id() >> 4;
-  f32x4_t s[2][NCT];
+// The waves of a head, whose accumulators and state are in LDS: the rows, if the share is all of the request, else its partial.
+template <int D, int NCT, bool F16, int NW>
+__device__ __forceinline__ void put_waves_together(const ShareParams& p, const MxLds<D, NCT, NW>& lds, const MxShare& x, int hg, const MxWave& w) {
+  constexpr int kQuads = D / 4;  // a thread's unit of work: 4 dims of one column
+  const int t16 = lane_id() & 15, kvh = hg * p.nwh + w.sub, ncols = x.r.q_len * p.group;
+  const int64_t row0 = ((int64_t)x.item * p.n_kv + kvh) * p.cols;
+  const Partials own(p.part_o + row0 * D, (uint32_t)(ncols * D * 4));
+  // Every wave's part of a quad is asked for before the first is used.  The lanes of a row of 16 work on one column: lane i has
+  // wave i's reference and sum, and its weight goes to the others by DPP.
+  auto with = [&](auto n_waves) {
+    constexpr int W = decltype(n_waves)::value;
+    for (int it = w.me; it < ncols * kQuads; it += w.threads) {
+      const int col = it / kQuads, d4 = (it - col * kQuads) * 4;
+      float2 ml = lds.state[w.sub * W + min(t16, W - 1)][col];
+      f32x4_t o[W];
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) s[u][ct] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int h = 0; h < D / 128; ++h) {
-      const float factor = block_factor<F16, true>(t.k_byte[h][u]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const u32x4_t k = mx_values8<F16>(t.k[h][u][c], factor);
-#pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) s[u][ct] = mfma_16x16x32_raw<F16>(k, c_.q[ct][4 * h + c], s[u][ct]);
+      for (int i = 0; i < W; ++i)
+        o[i] = *reinterpret_cast<const f32x4_t*>(&reinterpret_cast<const WavePart<D, NCT>*>(lds.wave[w.sub * W + i])->o[d4 >> 3][col * 8 + (d4 & 7)]);
+      if (t16 >= W) ml = float2{kNegInf, 0.f};
+      const float top = row_max16(ml.x), m = top == kNegInf ? 0.f : top;
+      const float e = fast_exp2(ml.x - m);  // 0 for a wave without visible keys
+      // a wave that saw nothing but NaN has no reference and a sum that is NaN, with any weight
+      const float l = row_sum16(e * ml.y);
+      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+      each([&](auto i) { acc += of_row_lane<decltype(i)::value>(e) * o[decltype(i)::value]; }, std::make_integer_sequence<int, W>{});
+      acc *= l > 0.f ? kBack<F16> / l : 0.f;  // (NaN: the accumulators are that too)
+      if (x.n_shares == 1) {
+        leave_quad<D, F16>(p, x.r, kvh, col, d4, acc);
+      } else {
+        own.store(16u * (uint32_t)it, acc);
+        // NaN: any weight above zero takes the partial's NaN into the merged row
+        if (d4 == 0)
+          __hip_atomic_store(p.part_lse + row0 + col, l > 0.f ? m + __log2f(l) : l == 0.f ? kNegInf : 0.f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
-  const bool need_mask = (tb < c_.all_lo) || (tb + 31 > c_.all_hi);
-  u32x4_t pb[NCT];
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    float x[8];  // of key tb + 8 g + of_group(n)
-#pragma unroll
-    for (int n = 0; n < 8; ++n) x[n] = s[n >> 2][ct][n & 3];
-    if (need_mask) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int key = tb + 8 * g + Place<D>::of_group(n);
-        if (key < c_.lo[ct] || key > c_.hi[ct]) x[n] = kNegInf;
-      }
-    }
-    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * p.scale_log2e;
-    // The reference moves only where a score is far beyond it: weights up to 2^kLazy are as exact as those up to 1
-    if (__any(mx > c_.top[ct] + kLazy)) {
-      const float top = fmaxf(c_.top[ct], max_across<32>(max_across<16>(mx)));
-      const float m = top == kNegInf ? 0.f : top;
-      const float alpha = fast_exp2(c_.top[ct] - m);
-      c_.top[ct] = top;
-      c_.m[ct] = m;
-      c_.l[ct] *= alpha;
-#pragma unroll
-      for (int h = 0; h < D / 128; ++h)
-#pragma unroll
-        for (int n = 0; n < 8; ++n) c_.o[ct][h][n] *= alpha;
-    }
-#pragma unroll
-    for (int n = 0; n < 8; ++n) x[n] = fast_exp2(__builtin_fmaf(x[n], p.scale_log2e, -c_.m[ct]));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pb[ct][i] = pack_16x2<F16>(x[2 * i], x[2 * i + 1]);
-      c_.l[ct] = add_weights<F16>(pb[ct][i], c_.l[ct]);  // the ones that multiply V
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < D / 128; ++h) {
-    u32x4_t v[8];
-#pragma unroll
-    for (int n = 0; n < 8; ++n) v[n] = mx_values8<F16>(t.v[h][n], block_factor<F16, false>(t.v_byte[h][n]));
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      u32x4_t vt;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t a = v[2 * i][n >> 1], b = v[2 * i + 1][n >> 1];
-        vt[i] = (n & 1) ? pack_hi16(a, b) : pack_lo16(a, b);
-      }
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) c_.o[ct][h][n] = mfma_16x16x32_raw<F16>(vt, pb[ct], c_.o[ct][h][n]);
-    }
-  }
-}
-
-// A wave's LDS: stages of codes and block bytes, and the slot ids of tiles to come.
-template <int D>
-struct WaveLds {
-  static constexpr int kAhead = D == 128 ? 3 : 1, kStages = kAhead + 1;    // tiles on their way while one is computed
-  static constexpr int kIdsAhead = kAhead + 1, kIdTiles = 2 * kStages;  // ids are asked for so many tiles before their tile is
-  static_assert((kStages & (kStages - 1)) == 0 && kIdTiles >= kAhead + kIdsAhead + 1);
-  static constexpr int kCodes = 32 * D, kScales = 32 * (D / 16), kStage = kCodes + kScales, kIds = kStages * kStage;
-  unsigned char bytes[kIds + kIdTiles * 256];
-};
-
-// At most N loads of the wave under way, and none of its reads of LDS: the stage that the next loads write has been read.
-template <int N>
-__device__ __forceinline__ void wait_tile() {
-  static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit field");
-  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
-  asm volatile("" ::: "memory");
-}
-
-// Keys [t_begin, t_end) of request `r`, in order, for the columns in `c_`; `lds`: the wave's own, so nobody else is waited for.
-// Everything comes by loads that write LDS, of which the compiler knows nothing: tile i is there when no more of them than those issued
-// behind its last are under way.  Each iteration issues the same number, in the same order: codes and block bytes of the tile kAhead on, ids of the tile kAhead +
-// kIdsAhead on.  Keys past the end are the last one again, and masked.
-template <int D, int NCT, bool F16, int WALK>
-__device__ __forceinline__ void attend_mx_keys(const SplitKvParams& p, const ReqInfo& r, int kvh, int t_begin, int t_end, unsigned char* lds,
-                                               MxColumns<D, NCT>& c_) {
-  using P = Place<D>;
-  using L = WaveLds<D>;
-  constexpr int kAhead = L::kAhead, kStages = L::kStages, kIdsAhead = L::kIdsAhead, kIdTiles = L::kIdTiles;
-  constexpr int kIssued = P::kLoads + P::kScaleLoads + 1;
-  constexpr int kScaleWords = D / 64;  // of 4 bytes, of a key
-  using Offset = typename std::conditional<(WALK & kWide) != 0, uint64_t, uint32_t>::type;
-  const int lane = lane_id(), t16 = lane & 15, g = lane >> 4, a = t16 >> 2, i = t16 & 3;
-  const unsigned char* codes = reinterpret_cast<const unsigned char*>(p.k_cache) + kvh * D;
-  const unsigned char* scales = reinterpret_cast<const unsigned char*>(p.v_cache) + kvh * (D / 16);
-  const int32_t* idx = p.kv_indices + r.kv_start + t_begin;
-  const int last = t_end - t_begin - 1, n_tiles = (last >> 5) + 1;
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)MSGL_LDS_PTR(unsigned char, lds));
-  const auto shared = MSGL_LDS_PTR(unsigned char, lds);
-  const uint32_t codes_stride = (uint32_t)p.k_stride0, scales_stride = (uint32_t)p.v_stride0;
-  auto offset = [](uint32_t slot, uint32_t stride) -> Offset {
-    if constexpr (WALK & kWide) return (uint64_t)slot * stride;
-    else return __umul24(slot, stride);  // both below 2^24 here
   };
-
-  const int j = lane / P::kLanes, piece = lane % P::kLanes;
-  auto send_ids = [&](int tile) {
-    lds_direct_b32(lds0 + L::kIds + (uint32_t)(tile & (kIdTiles - 1)) * 256u, idx, (uint32_t)min(tile * 32 + (lane & 31), last) * 4u);
-  };
-  auto send_tile = [&](int tile) {
-    const uint32_t stage = lds0 + (uint32_t)(tile & (kStages - 1)) * L::kStage;
-    const auto ids = shared + L::kIds + (tile & (kIdTiles - 1)) * 256;
-    uint32_t slot[P::kLoads];
-#pragma unroll
-    for (int q = 0; q < P::kLoads; q += 4) {
-      const u32x4_t four = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(ids + P::key(q, j) * 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) slot[q + e] = min(four[e], p.max_slot);
-    }
-    uint32_t scale_slot[P::kScaleLoads];
-#pragma unroll
-    for (int q = 0; q < P::kScaleLoads; ++q)
-      scale_slot[q] = min(*reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(ids + ((64 / kScaleWords) * q + lane / kScaleWords) * 4), p.max_slot);
-#pragma unroll
-    for (int u = 0; u < P::kLoads; ++u) {
-      const Offset from = offset(slot[u], codes_stride) + (uint32_t)((piece ^ P::turn(P::key(u, j))) * 16);
-      if constexpr (WALK & kStream) lds_stream_b128(stage + u * 1024u, codes, from);
-      else lds_direct_b128(stage + u * 1024u, codes, from);
-    }
-#pragma unroll
-    for (int q = 0; q < P::kScaleLoads; ++q)
-      lds_direct_b32(stage + L::kCodes + q * 256u, scales, offset(scale_slot[q], scales_stride) + (uint32_t)(lane % kScaleWords) * 4u);
-  };
-  for (int tile = 0; tile < kIdsAhead; ++tile) send_ids(tile);
-  wait_all_vm();
-#pragma unroll
-  for (int tile = 0; tile < kAhead; ++tile) {
-    send_tile(tile);
-    send_ids(tile + kIdsAhead);
-  }
-  for (int tile = 0; tile < n_tiles; ++tile) {
-    wait_tile<(kAhead - 1) * kIssued + 1>();
-    send_tile(tile + kAhead);
-    send_ids(tile + kAhead + kIdsAhead);
-    const auto at = shared + (tile & (kStages - 1)) * L::kStage;
-    const auto k_at = at + P::k_lane(a, i, g), v_at = at + P::v_lane(a, i, g);
-    const auto kb_at = at + L::kCodes + P::k_byte(a, i, g), vb_at = at + L::kCodes + 8 * g * (D / 16) + D / 32 + a;
-    MxTile<D> t;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int h = 0; h < D / 128; ++h) {
-        t.k[h][u] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>((h == 0 ? k_at : at + P::k_lane_h(a, i, g)) + P::k_of(u));
-        t.k_byte[h][u] = kb_at[(P::of_group(4 * u) - P::of_group(0)) * (D / 16) + 4 * h];
-      }
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int h = 0; h < D / 128; ++h) {
-        t.v[h][n] = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(v_at + P::v_of(n, h));
-        t.v_byte[h][n] = vb_at[P::of_group(n) * (D / 16) + 4 * h];
-      }
-    compute_mx_tile<D, NCT, F16>(p, t, t_begin + tile * 32, c_);
-  }
-  wait_all_vm();  // what is still under way writes LDS that the next keys want
+  if (w.waves == 4) with(std::integral_constant<int, 4>{});
+  else if (w.waves == 2) with(std::integral_constant<int, 2>{});
+  else with(std::integral_constant<int, 1>{});
 }
 
-// A request's share is done: its rows, if the segment held all of it, else its partial.
-template <int D, int NCT, bool F16>
-__device__ __forceinline__ void leave_share(const SplitKvParams& p, const ReqInfo& r, int seg, int b, int kvh, bool whole, MxColumns<D, NCT>& c_) {
-  const int t16 = lane_id() & 15, g = lane_id() >> 4;
-  const int ncols = r.q_len * p.group;
+// The partials of all shares of a request, by log-sum-exp: its rows.
+template <int D, bool F16>
+__device__ __forceinline__ void put_shares_together(const ShareParams& p, const MxShare& x, int hg, const MxWave& w) {
+  constexpr int kQuads = D / 4;
+  const int t16 = lane_id() & 15, kvh = hg * p.nwh + w.sub, ncols = x.r.q_len * p.group, n_shares = x.n_shares;
+  const int64_t step = (int64_t)p.n_kv * p.cols;  // rows from one share to the next
+  const int64_t first = ((int64_t)(x.item - x.share) * p.n_kv + kvh) * p.cols;
+  const uint32_t step_bytes = (uint32_t)(step * (D * 4));
+  const Partials all(p.part_o + first * D, (uint32_t)n_shares * step_bytes);
+  const float* const lse_from = p.part_lse + first;
+  // U shares of Q quads at a time; the lanes of a row of 16 work on the same columns
+  auto with = [&](auto in_flight, auto quads) {
+    constexpr int U = decltype(in_flight)::value, Q = decltype(quads)::value;
+    const int n_quads = ncols * kQuads;
+    for (int it = w.me; it < n_quads; it += Q * w.threads) {
+      float top[Q], l[Q];
+      f32x4_t acc[Q];
 #pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    const float l = sum_across<32>(sum_across<16>(c_.l[ct]));
-    const float inv = (l > 0.f) ? kBack<F16> / l : 0.f;  // (NaN: the accumulators are that too)
-    const int col = ct * 16 + t16;
-    if (col >= ncols) continue;
-    if (whole) {
-      const int qi = query_of(p, col), hh = col - qi * p.group;
-      uint16_t* orow = p.out + ((int64_t)(r.q_start + qi) * p.n_q + kvh * p.group + hh) * D;
+      for (int q = 0; q < Q; ++q) {
+        top[q] = kNegInf;
+        l[q] = 0.f;
+        acc[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+      for (int s0 = 0; s0 < n_shares; s0 += U) {  // shares past the last one: the last again, not used; quads likewise
+        const int mine = min(s0 + min(t16, U - 1), n_shares - 1);
+        float lse[Q];
+        f32x4_t o[Q][U];
 #pragma unroll
-      for (int h = 0; h < D / 128; ++h)
+        for (int q = 0; q < Q; ++q) {
+          const int at = min(it + q * w.threads, n_quads - kQuads + (it & (kQuads - 1)));
+          lse[q] = __hip_atomic_load(lse_from + mine * step + at / kQuads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          u32x4_t w;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) w[n] = pack_16x2<F16>(c_.o[ct][h][2 * n][i] * inv, c_.o[ct][h][2 * n + 1][i] * inv);
-          st_global_b128(orow + h * 128 + (4 * g + i) * 8, w);
+          for (int u = 0; u < U; ++u) o[q][u] = all.load(16u * (uint32_t)at, (uint32_t)min(s0 + u, n_shares - 1) * step_bytes);
         }
-    } else {
-      const int64_t block = (int64_t)(seg + b) * p.n_kv + kvh;
 #pragma unroll
-      for (int h = 0; h < D / 128; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4_t w0, w1;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            w0[n] = c_.o[ct][h][n][i] * inv;
-            w1[n] = c_.o[ct][h][4 + n][i] * inv;
-          }
-          float* dst = p.part_o + partial_offset(block, p.cols, col, h * 128 + (4 * g + i) * 8, D);
-          *reinterpret_cast<f32x4_t*>(dst) = w0;
-          *reinterpret_cast<f32x4_t*>(dst + 4) = w1;
+        for (int q = 0; q < Q; ++q) {
+          if (t16 >= U || s0 + t16 >= n_shares) lse[q] = kNegInf;
+          const float now = fmaxf(top[q], row_max16(lse[q])), m = now == kNegInf ? 0.f : now;
+          const float old = fast_exp2(top[q] - m), e = fast_exp2(lse[q] - m);
+          acc[q] *= old;
+          l[q] = l[q] * old + row_sum16(e);
+          top[q] = now;
+          each([&](auto u) {
+            if (s0 + decltype(u)::value < n_shares) acc[q] += of_row_lane<decltype(u)::value>(e) * o[q][decltype(u)::value];
+          }, std::make_integer_sequence<int, U>{});
         }
-      // NaN: any weight above zero takes the partial's NaN into the merged row
-      if (g == 0) p.part_lse[block * p.cols + col] = l > 0.f ? c_.m[ct] + __log2f(l) : l == 0.f ? kNegInf : 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int at = it + q * w.threads, col = at / kQuads;
+        if (at < n_quads) leave_quad<D, F16>(p, x.r, kvh, col, (at - col * kQuads) * 4, acc[q] * (l[q] > 0.f ? 1.0f / l[q] : 0.f));
+      }
     }
-  }
+  };
+  using std::integral_constant;
+  if (n_shares <= 4) with(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  else if (n_shares <= 8) with(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+  else with(integral_constant<int, 16>{}, integral_constant<int, 1>{});
 }
 
 template <int D, int NCT, bool F16, int WALK, int NW>
-__global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1) void mxfp4_attention_kernel(MxParams p) {
-  __shared__ __attribute__((aligned(256))) WaveLds<D> lds[NW];
-  const int seg = blockIdx.x / p.head_groups;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kvh = (blockIdx.x - seg * p.head_groups) * p.nwh + wave;
-  int seg_len, total, b, vs;
-  if (!locate_segment(p, seg, &seg_len, &total, &b, &vs)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  vs = __builtin_amdgcn_readfirstlane(vs);
-  seg_len = __builtin_amdgcn_readfirstlane(seg_len);
-  total = __builtin_amdgcn_readfirstlane(total);
-  int vpos = seg * seg_len;
-  const int seg_end = min(vpos + seg_len, total);
-  while (vpos < seg_end && b < p.batch) {
-    const ReqInfo r = request_info(p, b);
-    const int vlen = r.hi - r.lo;
-    if (vpos >= vs + vlen) {  // no keys, or past them in the empty positions: on to the next request
-      vs += stream_length(p, vlen);
-      vpos = max(vpos, vs);
-      ++b;
-      continue;
-    }
-    const int t_begin = r.lo + (vpos - vs);
-    const int t_end = min(r.hi, t_begin + (seg_end - vpos));
-    if (t_begin == r.lo && kvh == 0 && lane_id() == 0) {
-      // the wave that starts a request tells the merge kernel where its partials are
-      const int s_first = vs / seg_len;
-      p.req_items[2 * b] = s_first;
-      p.req_items[2 * b + 1] = (vs + vlen - 1) / seg_len - s_first + 1;
-    }
-    MxColumns<D, NCT> c_;
-    start_mx_columns<D, NCT, F16>(p, r, kvh, t_end, c_);
-    attend_mx_keys<D, NCT, F16, WALK>(p, r, kvh, t_begin, t_end, lds[wave].bytes, c_);
-    leave_share<D, NCT, F16>(p, r, seg, b, kvh, t_begin == r.lo && t_end == r.hi, c_);
-    vpos += t_end - t_begin;
+__global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1) void mxfp4_attention_kernel(ShareParams p) {
+  using Lds = MxLds<D, NCT, NW>;
+  __shared__ __attribute__((aligned(256))) Lds lds;
+  const int t16 = lane_id() & 15, g = lane_id() >> 4;
+  const int item = blockIdx.x / p.head_groups, hg = blockIdx.x - item * p.head_groups;
+  MxShare x;
+  if (!find_mx_share(p, item, &x)) return;
+  unsigned long long* const word = p.counts + ((int64_t)x.b * p.head_groups + hg) * kCountWords;
+  if (x.n_shares > 1 && threadIdx.x == 0) open_count(word, p.nonce);
+  const MxWave w(p);
+  unsigned char* const mine = lds.wave[w.sub * w.waves + w.sw];
+  const MxRange keys(p, x, w);
+  if (keys.begin < keys.end) send_first_ids<D>(p, x.r, keys.begin, keys.end, mine);
+  const int ncols = x.r.q_len * p.group, kvh = hg * p.nwh + w.sub;
+  MxColumns<D, NCT> c_;
+  start_mx_columns<D, NCT, F16>(p, x.r, kvh, keys.end, c_);
+  if (keys.begin < keys.end) attend_mx_keys<D, NCT, F16, WALK>(p, x.r, kvh, keys.begin, keys.end, mine, c_);
+  // ---- the waves of a head meet in LDS
+  auto& part = *reinterpret_cast<WavePart<D, NCT>*>(mine);
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const float l = sum_across<32>(sum_across<16>(c_.l[ct]));
+    const int col = ct * 16 + t16;
+    if (col >= ncols) continue;
+    if (g == 0) lds.state[w.sub * w.waves + w.sw][col] = float2{c_.top[ct], l};
+#pragma unroll
+    for (int h = 0; h < D / 128; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4_t w0, w1;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          w0[n] = c_.o[ct][h][n][i];
+          w1[n] = c_.o[ct][h][4 + n][i];
+        }
+        float* dst = &part.o[h * 16 + 4 * g + i][col * 8];
+        *reinterpret_cast<f32x4_t*>(dst) = w0;
+        *reinterpret_cast<f32x4_t*>(dst + 4) = w1;
+      }
   }
+  __syncthreads();
+  put_waves_together<D, NCT, F16, NW>(p, lds, x, hg, w);
+  if (x.n_shares == 1) return;
+  wait_all_vm();  // this wave's partials are where every CU sees them
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = count_one(word, p.nonce) == x.n_shares - 1;
+    if (last) st_agent(word, 0ull);  // as of a launch that never happened: the next replay counts anew
+    lds.last = last;
+  }
+  __syncthreads();
+  if (lds.last) put_shares_together<D, F16>(p, x, hg, w);
 }
 
-template <int D, int NCT, bool F16>
-int launch_walk(const MxParams& p, hipStream_t stream) {
-  auto launch = [&](auto kernel) { return launch_kernel(kernel, dim3((unsigned)(p.n_seg * p.head_groups)), dim3(64 * p.nwh), stream, p); };
-  auto heads = [&](auto w) {
-    constexpr int WALK = decltype(w)::value;
-    return p.nwh == 4   ? launch(mxfp4_attention_kernel<D, NCT, F16, WALK, 4>)
-           : p.nwh == 2 ? launch(mxfp4_attention_kernel<D, NCT, F16, WALK, 2>)
-                        : launch(mxfp4_attention_kernel<D, NCT, F16, WALK, 1>);
+template <int D, int NCT, int NW, bool F16>
+int launch_walk(const ShareParams& p, int64_t units, hipStream_t stream) {
+  auto launch = [&](auto w) {
+    return launch_kernel(mxfp4_attention_kernel<D, NCT, F16, decltype(w)::value, NW>, dim3((unsigned)units), dim3(64 * NW), stream, p);
   };
-  return p.walk == (kStream | kWide) ? heads(std::integral_constant<int, kStream | kWide>{})
-         : p.walk == kStream         ? heads(std::integral_constant<int, kStream>{})
-         : p.walk == kWide           ? heads(std::integral_constant<int, kWide>{})
-                                     : heads(std::integral_constant<int, kNarrow>{});
+  return p.walk == (kStream | kWide) ? launch(std::integral_constant<int, kStream | kWide>{})
+         : p.walk == kStream         ? launch(std::integral_constant<int, kStream>{})
+         : p.walk == kWide           ? launch(std::integral_constant<int, kWide>{})
+                                     : launch(std::integral_constant<int, kNarrow>{});
 }
 
-constexpr int kMinSegment = 64;
-int heads_per_group(int64_t n_kv) { return n_kv % 4 == 0 ? 4 : n_kv % 2 == 0 ? 2 : 1; }
-int segments(int64_t total_kv, int64_t n_kv) {
-  const int64_t waves = (int64_t)device_cus() * 8;
-  return (int)std::max<int64_t>(1, std::min(waves / n_kv, (total_kv + kMinSegment - 1) / kMinSegment));
+// How a launch is cut: waves of a workgroup, kv heads of one, shares that fit on the card at once and the most that there can be.
+struct Plan {
+  int waves, heads, min_len;
+  int64_t shares, max_shares;
+};
+// Which of them, by what a launch takes for each, in us, of the average request:
+//   bytes     at 6 TB/s with 4 heads to a workgroup, whose lines lie side by side, in 1.25 of that with 2 and 1.7 with 1 (32 requests of 8 K keys, 8
+//             heads: 60.2, 74.5 and 97.8 us); 8 waves of 8 heads, 1 KiB a slot, are a little better still (59.0; 64 of 8 K 107.0, not 120.8)
+//   a wave    0.018 a key, where there is little else (one request of 2 K keys, 4 heads 13.7, 2 10.3, 1 8.6)
+//   the merge 2 a trip of the loop in put_shares_together(), of which the more heads a workgroup has the more shares there are and the fewer threads to a head (16 of 4 K
+//             keys, 64 columns: 4 heads 91.4, 1 head 57.7; 32 columns of head_dim 256 81.7 and 35.1)
+// In 26 launches of 1 to 256 requests, 2 MB to 1.2 GB, it took the fastest of the four or one that was no more than 4 % slower.
+Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, int64_t cols) {
+  const int64_t cus = device_cus();
+  Plan best{};
+  best.min_len = cols <= 16 ? 128 : 512;
+  float least = 0.f;
+  auto consider = [&](int waves, int heads, float rate) {
+    const int64_t shares = std::max<int64_t>(cus / (n_kv / heads), 1);
+    const float request = (float)keys / (float)batch;
+    const float len = std::max(request / std::max((float)shares / (float)batch, 1.f), (float)best.min_len);
+    const int n = std::max((int)(request / len + 0.5f), 1);
+    const float loops = (float)(cols * head_dim / 4) / (float)(64 * waves / heads) / (n <= 4 ? 4.f : n <= 8 ? 2.f : 1.f);
+    const float stream = std::max((float)(keys * n_kv * head_dim) * (17.f / 16.f / 6e6f) * rate, 0.018f * len * (float)heads / (float)waves);
+    const float cost = stream + (n > 1 ? 2.f * loops * std::ceil((float)n / 16.f) : 0.f);
+    if (best.waves != 0 && cost >= least) return;
+    least = cost;
+    best.waves = waves;
+    best.heads = heads;
+    best.shares = shares;
+  };
+  consider(4, 1, 1.7f);
+  if (n_kv % 2 == 0) consider(4, 2, 1.25f);
+  if (n_kv % 4 == 0) consider(4, 4, 1.f);
+  if (n_kv % 8 == 0 && head_dim == 128 && cols <= 32) consider(8, 8, 0.98f);  // (the LDS of a CU holds no 8 waves with more)
+  best.max_shares = best.shares + batch;
+  return best;
 }
+size_t counts_bytes(int64_t batch, int64_t n_kv) { return (size_t)(batch * n_kv) * kCountWords * sizeof(unsigned long long); }
 
 }  // namespace
 
 int64_t mxfp4_max_columns(int64_t head_dim) { return head_dim == 128 ? 64 : 32; }
 
-size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t total_kv, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend) {
-  return splitkv_workspace_bytes(batch, n_q, n_kv, head_dim, max_len_extend, segments(total_kv, n_kv));
+// For every plan: which one it is may depend on a window
+size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend) {
+  const int64_t cols = n_q / n_kv * max_len_extend, most = device_cus() + batch;
+  return counts_bytes(batch, n_kv) + (size_t)(most * n_kv * cols) * (size_t)(head_dim + 1) * sizeof(float);
 }
 
 int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   const int64_t n_kv = a.pool.n_kv, d = a.pool.head_dim, cols = a.n_q / n_kv * a.max_len_extend;
   if (cols < 1 || cols > mxfp4_max_columns(d)) return MSGL_ERR_SHAPE;
-  MxParams p{};
+  if (a.f16 && cols > 16) return MSGL_ERR_DTYPE;
+  const int64_t keys = visible_keys(a.batch, a.total_kv, a.window, a.max_len_extend, a.is_cross != 0);
+  const Plan plan = plan_of(a.batch, keys, n_kv, d, cols);
+  ShareParams p{};
   p.q = static_cast<const uint16_t*>(a.q);
-  p.k_cache = static_cast<const uint16_t*>(a.pool.codes);   // as bytes, strides too
+  p.k_cache = static_cast<const uint16_t*>(a.pool.codes);  // as bytes, strides too
   p.v_cache = static_cast<const uint16_t*>(a.pool.scales);
   p.k_stride0 = a.pool.codes_stride0;
   p.v_stride0 = a.pool.scales_stride0;
@@ -466,36 +412,46 @@ int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   p.group = (int32_t)(a.n_q / n_kv);
   p.per_group = 65535u / (uint32_t)p.group + 1u;
   p.cols = (int32_t)cols;
-  p.nwh = heads_per_group(n_kv);
-  p.head_groups = (int32_t)(n_kv / p.nwh);
-  p.n_seg = segments(a.total_kv, n_kv);
-  p.min_seg = kMinSegment;
   p.max_len_extend = p.q_cap = a.max_len_extend;
   p.f16 = a.f16;
   p.is_cross = a.is_cross;
   p.window = a.window;
   p.max_slot = (uint32_t)(a.pool.num_slots - 1);
   p.negate = a.sm_scale < 0.f ? -1 : a.sm_scale == 0.f ? 1 : 0;
-  p.scale_log2e = a.sm_scale == 0.f ? 1.f : fabsf(a.sm_scale) * kLog2e * (a.f16 ? 2.f : 1.f);
-  const int64_t rows = ((int64_t)p.n_seg + a.batch) * n_kv * cols;
-  char* ws = static_cast<char*>(a.workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  p.part_lse = reinterpret_cast<float*>(ws + (size_t)rows * d * sizeof(float));
-  p.req_items = reinterpret_cast<int32_t*>(ws + (size_t)rows * (d + 1) * sizeof(float));
-  const int nct = (int)((cols + 15) / 16);
-  if (a.f16 && nct > 1) return MSGL_ERR_DTYPE;
+  p.scale_log2e = a.sm_scale == 0.f ? 1.f : std::fabs(a.sm_scale) * kLog2e * (a.f16 ? 2.f : 1.f);
   const int64_t stride = std::max(a.pool.codes_stride0, a.pool.scales_stride0);
   const bool wide = a.pool.num_slots > 1 << 24 || stride >= 1 << 24 || (uint64_t)a.pool.num_slots * (uint64_t)stride >= (1ull << 32);
-  const int64_t keys = visible_keys(a.batch, a.total_kv, a.window, a.max_len_extend, a.is_cross != 0);
   p.walk = (wide ? kWide : kNarrow) | (streams(keys * n_kv * (d + d / 16)) ? kStream : kNarrow);
-  const int rc = d == 128 ? (a.f16      ? launch_walk<128, 1, true>(p, stream)
-                             : nct == 1 ? launch_walk<128, 1, false>(p, stream)
-                             : nct == 2 ? launch_walk<128, 2, false>(p, stream)
-                                        : launch_walk<128, 4, false>(p, stream))
-                          : (a.f16      ? launch_walk<256, 1, true>(p, stream)
-                             : nct == 1 ? launch_walk<256, 1, false>(p, stream)
-                                        : launch_walk<256, 2, false>(p, stream));
-  return rc != MSGL_OK ? rc : launch_fp32_merge(p, d, stream);
+  p.nwh = plan.heads;
+  p.head_groups = (int32_t)(n_kv / plan.heads);
+  p.shares = (int32_t)plan.shares;
+  p.min_len = (float)plan.min_len;
+  p.wave_shift = __builtin_ctz((unsigned)(plan.waves / plan.heads));
+  p.counts = static_cast<unsigned long long*>(a.workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + counts_bytes(a.batch, n_kv));
+  p.part_lse = p.part_o + (size_t)plan.max_shares * (size_t)(n_kv * cols) * (size_t)d;
+  p.nonce = next_launch_number();
+  const int64_t units = plan.max_shares * p.head_groups;
+  if (units > 0x7fffffffLL) return MSGL_ERR_SHAPE;
+  const int nct = (int)((cols + 15) / 16);
+  auto launch = [&](auto dim, auto tiles, auto half) {
+    constexpr int D = decltype(dim)::value, NCT = decltype(tiles)::value;
+    constexpr bool F16 = decltype(half)::value;
+    if constexpr (D == 128 && NCT <= 2) {
+      if (plan.waves == 8) return launch_walk<D, NCT, 8, F16>(p, units, stream);
+    }
+    return launch_walk<D, NCT, 4, F16>(p, units, stream);
+  };
+  using std::integral_constant;
+  if (d == 128) {
+    if (a.f16) return launch(integral_constant<int, 128>{}, integral_constant<int, 1>{}, std::true_type{});
+    if (nct == 1) return launch(integral_constant<int, 128>{}, integral_constant<int, 1>{}, std::false_type{});
+    if (nct == 2) return launch(integral_constant<int, 128>{}, integral_constant<int, 2>{}, std::false_type{});
+    return launch(integral_constant<int, 128>{}, integral_constant<int, 4>{}, std::false_type{});
+  }
+  if (a.f16) return launch(integral_constant<int, 256>{}, integral_constant<int, 1>{}, std::true_type{});
+  if (nct == 1) return launch(integral_constant<int, 256>{}, integral_constant<int, 1>{}, std::false_type{});
+  return launch(integral_constant<int, 256>{}, integral_constant<int, 2>{}, std::false_type{});
 }
 
 }  // namespace msgl

@@ -27,6 +27,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "agent_scope.h"
 #include "launch_number.h"
 #include "new_token.h"
 
@@ -75,26 +76,6 @@ __device__ __forceinline__ int ceil_div(int a, int b) {
   return q;
 }
 
-__device__ __forceinline__ void st_agent(unsigned long long* p, unsigned long long v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ unsigned long long ld_agent(const unsigned long long* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// 16 bytes of the partials at agent scope.  (As two 8-byte accesses, the largest there are of atomics, each of them walks all
-// the lines that the wave's 16-byte pieces lie in: 24 loads of a thread took 1.5 K cycles to be issued, 48 of head_dim 256 3.8 K.)
-constexpr int kAgentScope = 16;  // sc1
-struct Partials {
-  __amdgpu_buffer_rsrc_t at;
-  __device__ __forceinline__ Partials(float* from, uint32_t bytes) : at(__builtin_amdgcn_make_buffer_rsrc(from, 0, bytes, 0x00020000)) {}
-  __device__ __forceinline__ f32x4_t load(uint32_t lane_at, uint32_t share_at) const {
-    return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(at, (int)lane_at, (int)share_at, kAgentScope));
-  }
-  __device__ __forceinline__ void store(uint32_t lane_at, f32x4_t v) const {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), at, (int)lane_at, 0, kAgentScope);
-  }
-};
 template <typename F, int... I>
 __device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);

@@ -42,7 +42,6 @@
 #include <type_traits>
 
 #include "new_token.h"
-#include "splitkv_stream.h"
 
 namespace msgl {
 namespace {
@@ -71,6 +70,85 @@ __device__ __forceinline__ uint32_t pack_half2_clamped(float lo, float hi) {
   v[0] = (_Float16)__builtin_fminf(__builtin_fmaxf(lo, -65504.f), 65504.f);
   v[1] = (_Float16)__builtin_fminf(__builtin_fmaxf(hi, -65504.f), 65504.f);
   return __builtin_bit_cast(uint32_t, v);
+}
+
+// Where dim `dim` of column `col` of the partial of (item, kv head) number `block` lives.  Blocks
+// of 8 dims are the outer index and columns the inner one: in the attention kernel's accumulator
+// layout the 16 lanes of a row group hold the same 8 dims of 16 consecutive columns, so one store
+// instruction writes 32 contiguous bytes per lane and 512 contiguous bytes per row group.  (With
+// the column as the outer index every lane of a store wrote 16 bytes of a different 512-byte row:
+// 64 partial cache lines per instruction, and the partial stores of a share cost as much as
+// several microseconds of streaming.)
+__device__ __forceinline__ int64_t partial_offset(int64_t block, int cols, int col, int dim, int D) {
+  return (block * cols * (int64_t)D) + ((int64_t)(dim >> 3) * cols + col) * 8 + (dim & 7);
+}
+
+// A request with visible keys takes their number of positions in the stream plus `boundary`
+// positions without tokens behind them.  Starting on the next request costs a workgroup a fixed
+// time (its geometry, Q rows, slot ids and first tiles are three dependent memory round trips, and
+// the load pipeline drains and refills): measured 8-9 us, the time of about a hundred tokens, and the
+// kernel ends when its slowest workgroup does.  Charging the boundary to the segment that crosses it
+// gives that workgroup fewer tokens; a segment that ends or starts inside the empty positions just
+// has less to do or starts at the next request.
+__device__ __forceinline__ int stream_length(const SplitKvParams& p, int visible) {
+  return visible > 0 ? visible + p.boundary : 0;
+}
+
+// Segments are a multiple of 64 positions long, one trip of the tile loop.  (Multiples of 16 or 32
+// fill the last few segments that rounding up to 64 leaves without work, but give every share a
+// partly filled trip: measured 0.5-1 % slower on the decode and verify shapes.)
+__device__ __forceinline__ int segment_length(int total, int n_seg, int min_seg) {
+  const int even = ((total + n_seg - 1) / n_seg + 63) / 64 * 64;
+  return max(even, min_seg);
+}
+
+// Wave-cooperative: length of the stream, and the request that holds stream position
+// `seg * seg_len` (its keys or the empty positions behind them) together with the stream position
+// of that request's first key.
+// Returns false when the segment starts beyond the stream.  All lanes must call.
+__device__ __forceinline__ bool locate_segment(const SplitKvParams& p, int seg, int* seg_len,
+                                               int* total_out, int* req, int* req_vstart) {
+  const int lane = lane_id();
+  int total = 0, n = 0, incl = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kWave) {
+    const int b = b0 + lane;
+    n = 0;
+    if (b < p.batch) {
+      const ReqInfo r = request_info(p, b);
+      n = stream_length(p, r.hi - r.lo);
+    }
+    incl = wave_inclusive_scan(n);
+    total += __shfl(incl, kWave - 1, kWave);
+  }
+  total = max(total - p.boundary, 0);  // nothing follows the last request: its empty positions go
+  const int len = segment_length(total, p.n_seg, p.min_seg);
+  *seg_len = len;
+  *total_out = total;
+  const int pos = seg * len;
+  if (pos >= total) return false;
+  int base = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kWave) {
+    if (p.batch > kWave) {  // more than one batch of requests: recompute this batch
+      const int b = b0 + lane;
+      n = 0;
+      if (b < p.batch) {
+        const ReqInfo r = request_info(p, b);
+        n = stream_length(p, r.hi - r.lo);
+      }
+      incl = wave_inclusive_scan(n);
+    }
+    const int batch_total = __shfl(incl, kWave - 1, kWave);
+    if (pos < base + batch_total) {
+      const int first = base + incl - n;
+      const bool hit = (pos >= first) && (pos < first + n);
+      const int src = __ffsll((long long)__ballot(hit)) - 1;
+      *req = b0 + src;
+      *req_vstart = __shfl(first, src, kWave);
+      return true;
+    }
+    base += batch_total;
+  }
+  return false;
 }
 
 template <int D, int NCT, int NW>
@@ -534,21 +612,6 @@ int launch_attn(const SplitKvParams& p, hipStream_t stream) {
   return launch(std::false_type{}, New<kStored>{});
 }
 
-template <int D, bool kF32>  // of bf16 launches' partials
-int launch_merge(const SplitKvParams& p, hipStream_t stream) {
-  const dim3 mgrid((unsigned)(p.batch * p.max_len_extend), (unsigned)p.n_q);
-  // four waves per row when a request can be cut into more items than one wave takes in a trip
-  // and the rows are few enough that the extra waves cost nothing
-  constexpr int kItemsPerTrip = kWave / (D / 8) * (1 + kMergeUnroll);
-  const bool wide_merge = p.n_seg > kItemsPerTrip && (int64_t)mgrid.x * mgrid.y <= 1024;
-  if (wide_merge) {
-    return launch_kernel(p.f16 ? splitkv_merge_kernel<D, true, true> : splitkv_merge_kernel<D, false, kF32>, mgrid, dim3(64 * kMergeWaves), stream, p);
-  }
-  constexpr unsigned kRows = kMergeWaves * (kWave / (D / 8));  // of a workgroup
-  const dim3 rows(mgrid.x, (mgrid.y + kRows - 1) / kRows);
-  return launch_kernel(p.f16 ? splitkv_merge_rows_kernel<D, true, true> : splitkv_merge_rows_kernel<D, false, kF32>, rows, dim3(64 * kMergeWaves), stream, p);
-}
-
 template <int D, int NCT>
 int launch_dn(const SplitKvParams& p, int waves, hipStream_t stream) {
   if ((p.f16 || p.nt.k != nullptr) && NCT != 1) return MSGL_ERR_DTYPE;
@@ -560,7 +623,18 @@ int launch_dn(const SplitKvParams& p, int waves, hipStream_t stream) {
     if (waves == 8) rc = launch_attn<D, NCT, 8>(p, stream);
   }
   if (rc != MSGL_OK) return rc;
-  return launch_merge<D, fp32_partials<D, NCT, false>()>(p, stream);
+  const dim3 mgrid((unsigned)(p.batch * p.max_len_extend), (unsigned)p.n_q);
+  // four waves per row when a request can be cut into more items than one wave takes in a trip
+  // and the rows are few enough that the extra waves cost nothing
+  constexpr int kItemsPerTrip = kWave / (D / 8) * (1 + kMergeUnroll);
+  const bool wide_merge = p.n_seg > kItemsPerTrip && (int64_t)mgrid.x * mgrid.y <= 1024;
+  constexpr bool kF32 = fp32_partials<D, NCT, false>();
+  if (wide_merge) {
+    return launch_kernel(p.f16 ? splitkv_merge_kernel<D, true, true> : splitkv_merge_kernel<D, false, kF32>, mgrid, dim3(64 * kMergeWaves), stream, p);
+  }
+  constexpr unsigned kRows = kMergeWaves * (kWave / (D / 8));  // of a workgroup
+  const dim3 rows(mgrid.x, (mgrid.y + kRows - 1) / kRows);
+  return launch_kernel(p.f16 ? splitkv_merge_rows_kernel<D, true, true> : splitkv_merge_rows_kernel<D, false, kF32>, rows, dim3(64 * kMergeWaves), stream, p);
 }
 
 // How a shape's column tiles map onto waves: tiles per wave and waves per kv head.
@@ -735,10 +809,6 @@ void fill_splitkv_params(const SplitKvArgs& a, SplitKvParams& p) {
   const int64_t keys = visible_keys(a.batch, a.total_kv, a.window, a.max_len_extend, a.is_cross != 0);
   const bool once = col_split(nct_for(p.cols), a.head_dim, a.total_kv, a.n_kv).col_waves == 1;
   p.walk = (once && streams(keys * a.n_kv * a.head_dim * 4) ? kStream : kNarrow) | (pool_bytes >= (1ull << 32) ? kWide : kNarrow);
-}
-
-int launch_fp32_merge(const SplitKvParams& p, int64_t head_dim, hipStream_t stream) {
-  return head_dim == 128 ? launch_merge<128, true>(p, stream) : launch_merge<256, true>(p, stream);
 }
 
 int launch_splitkv(const SplitKvArgs& a, const NewTokens& n, hipStream_t stream) {
