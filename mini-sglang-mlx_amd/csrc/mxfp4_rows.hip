@@ -8,6 +8,7 @@ namespace msgl {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnpackRows = 4;  // of a thread, on their way at once
 
 __device__ __forceinline__ float value16(uint32_t w, int half, bool f16) {
   const uint32_t h = half ? w >> 16 : w & 0xffffu;
@@ -111,14 +112,30 @@ __global__ __launch_bounds__(kThreads) void unpack_mxfp4_kernel(UnpackParams p) 
     end = min((int64_t)p.kv_indptr[b + 1], end);
     begin = start + (max(p.prefix_lens[b] - p.window + 1, 0) & ~127);
   }
-  const int64_t items = max(end - begin, (int64_t)0) * p.n_kv;
-  for (int64_t at = first * kAtOnce + threadIdx.x / kLanes; at < items; at += step * kAtOnce) {
-    const int64_t row = begin + at / p.n_kv, head = at % p.n_kv;
-    const int64_t slot = min((uint32_t)p.kv_indices[row], p.max_slot);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(p.codes + slot * p.codes_stride + head * D + lane * 4);
-    const uint32_t byte = p.scales[slot * p.scales_stride + head * (D / 16) + (lane >> 2)];
-    st_global_b128((of_v ? p.v : p.k) + (row * p.n_kv + head) * D + j * 8, mx_values8<false>(codes, mx_scale(byte)));
-    if (head == 0 && lane == 0) p.numbers[row] = (int32_t)row;
+  const uint32_t items = (uint32_t)max(end - begin, (int64_t)0) * p.n_kv;
+  for (uint32_t at0 = (uint32_t)first * kAtOnce * kUnpackRows + threadIdx.x / kLanes; at0 < items; at0 += (uint32_t)step * kAtOnce * kUnpackRows) {
+    uint32_t row[kUnpackRows], head[kUnpackRows], codes[kUnpackRows], byte[kUnpackRows];
+#pragma unroll
+    for (int u = 0; u < kUnpackRows; ++u) {
+      const uint32_t at = min(at0 + u * kAtOnce, items - 1);
+      const uint32_t r = at / p.n_kv;
+      row[u] = (uint32_t)begin + r;
+      head[u] = at - r * p.n_kv;
+    }
+    uint32_t slot[kUnpackRows];
+#pragma unroll
+    for (int u = 0; u < kUnpackRows; ++u) slot[u] = min((uint32_t)p.kv_indices[row[u]], p.max_slot);
+#pragma unroll
+    for (int u = 0; u < kUnpackRows; ++u) {
+      codes[u] = *reinterpret_cast<const uint32_t*>(p.codes + slot[u] * p.codes_stride + head[u] * D + lane * 4);
+      byte[u] = p.scales[slot[u] * p.scales_stride + head[u] * (D / 16) + (lane >> 2)];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnpackRows; ++u) {
+      if (at0 + u * kAtOnce >= items) break;
+      st_global_b128((of_v ? p.v : p.k) + ((int64_t)row[u] * p.n_kv + head[u]) * D + j * 8, mx_values8<false>(codes[u], mx_scale(byte[u])));
+      if (head[u] == 0 && lane == 0) p.numbers[row[u]] = (int32_t)row[u];
+    }
   }
 }
 
@@ -141,7 +158,8 @@ int launch_unpack_mxfp4(const Mxfp4UnpackArgs& a, hipStream_t stream) {
   p.window = a.window;
   p.n_kv = (uint32_t)a.pool.n_kv;
   p.max_slot = (uint32_t)(a.pool.num_slots - 1);
-  const int64_t at_once = kThreads / (a.pool.head_dim / 4), most = 16 * (int64_t)device_cus();
+  if (a.total_kv * a.pool.n_kv > 0x7fffffffLL) return MSGL_ERR_SHAPE;
+  const int64_t at_once = kUnpackRows * (kThreads / (a.pool.head_dim / 4)), most = 16 * (int64_t)device_cus();
   auto blocks = [&](int64_t keys) { return std::max<int64_t>(1, (keys * a.pool.n_kv + at_once - 1) / at_once); };
   int64_t grid = std::min(blocks(a.total_kv), most);
   if (a.window > 0) {
