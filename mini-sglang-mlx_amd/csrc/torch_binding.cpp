@@ -844,9 +844,9 @@ PyObject* load_kv_cache_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n_arg
     {
       NoGil nogil;
       OnDevice on(dev);
-      const Tensor both = empty({2, length, n_kv, d}, half ? at::kHalf : at::kBFloat16, dev), ix = idx.contiguous();
-      k = both.select(0, 0);
-      v = both.select(0, 1);
+      const Tensor ix = idx.contiguous();
+      k = empty({length, n_kv, d}, half ? at::kHalf : at::kBFloat16, dev);
+      v = empty({length, n_kv, d}, half ? at::kHalf : at::kBFloat16, dev);
       rc = msgl_load_kv_cache_mxfp4(codes.data_ptr(), scales.data_ptr(), ints(ix), k.data_ptr(), v.data_ptr(), length, n_kv, d, codes.size(0),
                                     page_stride(codes), page_stride(scales), half ? MSGL_DTYPE_F16 : MSGL_DTYPE_BF16, on.ptr());
     }
