@@ -4,10 +4,10 @@
 // workgroup take a head each, or cut a head's share again and meet in LDS; and of a request that several shares hold the workgroup that counts last puts
 // the partials together.  One launch, and nobody waits for anybody: a merge in a launch of its own took 8 us of small calls and 12 of 32 requests of 32 columns,
 // and equal parts of the stream of all keys, which begin and end inside requests, as long as whole shares or longer (64 requests of 8 K keys 109
-// us against 107, 8 of 4 K 18.7 against 16.3).  Partials and counts travel at agent scope; a count word carries the launch's number
+// us against 107, 8 of 4 K 18.7 against 15.5).  Partials and counts travel at agent scope; a count word carries the launch's number
 // (launch_number.h), so the workspace needs no clearing, and is left as of a launch that never happened, so a replay counts anew.
 //
-// Bound by memory: 16 requests of 32-128 K keys of 8 heads of 128, 6.0 TB/s; 64 of 512-8 K 5.3.
+// Bound by memory: 16 requests of 32-128 K keys of 8 heads of 128, 6.3 TB/s; 64 of 512-8 K 5.5.
 #include <cmath>
 #include <utility>
 
@@ -344,8 +344,8 @@ struct Plan {
   int64_t shares, max_shares;
 };
 // Which of them, by what a launch takes for each, in us, of the average request:
-//   bytes     at 6 TB/s with 4 heads to a workgroup, whose lines lie side by side, in 1.25 of that with 2 and 1.7 with 1 (32 requests of 8 K keys, 8
-//             heads: 60.2, 74.5 and 97.8 us); 8 waves of 8 heads, 1 KiB a slot, are a little better still (59.0; 64 of 8 K 107.0, not 120.8)
+//   bytes     at 6 TB/s with 4 heads to a workgroup, whose lines lie side by side, in 1.25 of that with 2 and 1.7 with 1; 8 waves of 8 heads, 1 KiB a slot, are
+//             faster still (16 requests of 64 K keys, 8 heads: 200 us with 8, 220 with 4, 259 with 2, 379 with 1)
 //   a wave    0.018 a key, where there is little else (one request of 2 K keys, 4 heads 13.7, 2 10.3, 1 8.6)
 //   the merge 2 a trip of the loop in put_shares_together(), of which the more heads a workgroup has the more shares there are and the fewer threads to a head (16 of 4 K
 //             keys, 64 columns: 4 heads 91.4, 1 head 57.7; 32 columns of head_dim 256 81.7 and 35.1)
@@ -372,7 +372,7 @@ Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, int64_
   consider(4, 1, 1.7f);
   if (n_kv % 2 == 0) consider(4, 2, 1.25f);
   if (n_kv % 4 == 0) consider(4, 4, 1.f);
-  if (n_kv % 8 == 0 && head_dim == 128 && cols <= 32) consider(8, 8, 0.98f);  // (the LDS of a CU holds no 8 waves with more)
+  if (n_kv % 8 == 0 && head_dim == 128 && cols <= 32) consider(8, 8, 0.93f);  // (with more columns 8 waves' accumulators are no room for)
   best.max_shares = best.shares + batch;
   return best;
 }
