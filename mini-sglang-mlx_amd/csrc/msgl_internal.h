@@ -289,8 +289,7 @@ struct Mxfp4AttentionArgs {
   float sm_scale;
   int32_t max_len_extend, is_cross, window, f16;
 };
-// most columns (queries of a request times q heads of a kv head) of a launch
-int64_t mxfp4_max_columns(int64_t head_dim);
+bool mxfp4_reads_codes(int64_t group, int64_t head_dim, int64_t max_len_extend);
 size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend);
 int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream);
 

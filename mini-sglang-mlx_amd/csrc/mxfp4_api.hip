@@ -37,7 +37,7 @@ Unpacked unpacked(int64_t total_kv, int64_t n_kv, int64_t d) {
   const size_t rows = whole((size_t)total_kv * n_kv * d * 2);
   return Unpacked{0, rows, 2 * rows, 2 * rows + whole((size_t)total_kv * sizeof(int32_t))};
 }
-bool reads_pool(int64_t n_q, int64_t n_kv, int64_t d, int64_t max_len_extend) { return n_q / n_kv * max_len_extend <= msgl::mxfp4_max_columns(d); }
+bool reads_pool(int64_t n_q, int64_t n_kv, int64_t d, int64_t max_len_extend) { return msgl::mxfp4_reads_codes(n_q / n_kv, d, max_len_extend); }
 
 }  // namespace
 

@@ -19,7 +19,7 @@ namespace msgl {
 namespace {
 
 struct ShareParams : MxParams {
-  unsigned long long* counts;     // [batch][head_groups][kCountWords]: shares done
+  unsigned long long* counts;     // [query block][batch][head_groups][kCountWords]: shares done
   unsigned long long nonce;       // launch_number.h
   int32_t shares;                 // as many as there may be ..
   float min_len;                  // .. if that makes none shorter
@@ -42,7 +42,7 @@ __device__ __forceinline__ int shares_of(int visible, float per_len) { return (i
 // All lanes must call; false past the last share.
 __device__ __forceinline__ bool find_mx_share(const ShareParams& p, int item, MxShare* x) {
   const int lane = lane_id();
-  auto visible_of = [&](const ReqInfo& r, int b0) { return b0 + lane < p.batch ? max(r.hi - r.lo, 0) : 0; };
+  auto visible_of = [&](const ReqInfo& r, int b0) { return b0 + lane < p.batch && r.q_len > 0 ? max(r.hi - r.lo, 0) : 0; };
   auto request_at = [&](int b0) { return request_info(p, min(b0 + lane, p.batch - 1)); };
   const ReqInfo first64 = request_at(0);
   int visible[kCached / kWave];
@@ -94,7 +94,7 @@ __device__ __forceinline__ bool find_mx_share(const ShareParams& p, int item, Mx
     x->b = b0 + src;
     x->share = item - __builtin_amdgcn_readlane(first, src);
     x->n_shares = __builtin_amdgcn_readlane(n, src);
-    x->item = item;
+    x->item = blockIdx.y * (gridDim.x / p.head_groups) + item;
     return true;
   };
   if (here(visible[0], 0, [&](int src) {
@@ -277,10 +277,11 @@ __global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1
   using Lds = MxLds<D, NCT, NW>;
   __shared__ __attribute__((aligned(256))) Lds lds;
   const int t16 = lane_id() & 15, g = lane_id() >> 4;
+  p.q_begin = blockIdx.y * p.max_len_extend;
   const int item = blockIdx.x / p.head_groups, hg = blockIdx.x - item * p.head_groups;
   MxShare x;
   if (!find_mx_share(p, item, &x)) return;
-  unsigned long long* const word = p.counts + ((int64_t)x.b * p.head_groups + hg) * kCountWords;
+  unsigned long long* const word = p.counts + (((int64_t)blockIdx.y * p.batch + x.b) * p.head_groups + hg) * kCountWords;
   if (x.n_shares > 1 && threadIdx.x == 0) open_count(word, p.nonce);
   const MxWave w(p);
   unsigned char* const mine = lds.wave[w.sub * w.waves + w.sw];
@@ -328,15 +329,27 @@ __global__ __launch_bounds__(64 * NW, (D == 128 && NCT <= 2) || NCT == 1 ? 2 : 1
 }
 
 template <int D, int NCT, int NW, bool F16>
-int launch_walk(const ShareParams& p, int64_t units, hipStream_t stream) {
+int launch_walk(const ShareParams& p, dim3 grid, hipStream_t stream) {
   auto launch = [&](auto w) {
-    return launch_kernel(mxfp4_attention_kernel<D, NCT, F16, decltype(w)::value, NW>, dim3((unsigned)units), dim3(64 * NW), stream, p);
+    return launch_kernel(mxfp4_attention_kernel<D, NCT, F16, decltype(w)::value, NW>, grid, dim3(64 * NW), stream, p);
   };
   return p.walk == (kStream | kWide) ? launch(std::integral_constant<int, kStream | kWide>{})
          : p.walk == kStream         ? launch(std::integral_constant<int, kStream>{})
          : p.walk == kWide           ? launch(std::integral_constant<int, kWide>{})
                                      : launch(std::integral_constant<int, kNarrow>{});
 }
+
+// Columns that a workgroup's waves hold, and the blocks of queries, with all their q heads of a kv head, that a request's are cut into: each reads the keys anew.
+constexpr int64_t most_columns(int64_t head_dim) { return head_dim == 128 ? 64 : 32; }
+struct QueryBlocks {
+  int64_t blocks, queries, cols;  // queries and columns of one
+  QueryBlocks(int64_t group, int64_t head_dim, int64_t max_len_extend) {
+    const int64_t most = std::max<int64_t>(most_columns(head_dim) / group, 1);
+    blocks = (max_len_extend + most - 1) / most;
+    queries = (max_len_extend + blocks - 1) / blocks;
+    cols = queries * group;
+  }
+};
 
 // How a launch is cut: waves of a workgroup, kv heads of one, shares that fit on the card at once and the most that there can be.
 struct Plan {
@@ -346,54 +359,63 @@ struct Plan {
 // Which of them, by what a launch takes for each, in us, of the average request:
 //   bytes     at 6 TB/s with 4 heads to a workgroup, whose lines lie side by side, in 1.25 of that with 2 and 1.7 with 1; 8 waves of 8 heads, 1 KiB a slot, are
 //             faster still (16 requests of 64 K keys, 8 heads: 200 us with 8, 220 with 4, 259 with 2, 379 with 1)
-//   a wave    0.018 a key, where there is little else (one request of 2 K keys, 4 heads 13.7, 2 10.3, 1 8.6)
+//   a wave    0.018 a key of 16 columns of 128, where there is little else (one request of 2 K keys, 4 heads 13.7, 2 10.3, 1 8.6)
 //   the merge 2 a trip of the loop in put_shares_together(), of which the more heads a workgroup has the more shares there are and the fewer threads to a head (16 of 4 K
 //             keys, 64 columns: 4 heads 91.4, 1 head 57.7; 32 columns of head_dim 256 81.7 and 35.1)
 // In 26 launches of 1 to 256 requests, 2 MB to 1.2 GB, it took the fastest of the four or one that was no more than 4 % slower.
-Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, int64_t cols) {
-  const int64_t cus = device_cus();
+Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, const QueryBlocks& q) {
+  const int64_t cus = device_cus(), cols = q.cols;
+  const float wave_key = 0.018f * (0.5f + 0.5f * (float)((cols + 15) / 16 * head_dim / 128));
   Plan best{};
-  best.min_len = cols <= 16 ? 128 : 512;
   float least = 0.f;
-  auto consider = [&](int waves, int heads, float rate) {
-    const int64_t shares = std::max<int64_t>(cus / (n_kv / heads), 1);
+  auto consider = [&](int waves, int heads, float rate, int min_len) {
+    const int64_t shares = std::max<int64_t>(cus / (n_kv / heads * q.blocks), 1);
     const float request = (float)keys / (float)batch;
-    const float len = std::max(request / std::max((float)shares / (float)batch, 1.f), (float)best.min_len);
+    const float len = std::max(request / std::max((float)shares / (float)batch, 1.f), (float)min_len);
     const int n = std::max((int)(request / len + 0.5f), 1);
     const float loops = (float)(cols * head_dim / 4) / (float)(64 * waves / heads) / (n <= 4 ? 4.f : n <= 8 ? 2.f : 1.f);
-    const float stream = std::max((float)(keys * n_kv * head_dim) * (17.f / 16.f / 6e6f) * rate, 0.018f * len * (float)heads / (float)waves);
+    const float stream = std::max((float)(keys * n_kv * head_dim * q.blocks) * (17.f / 16.f / 6e6f) * rate, wave_key * len * (float)heads / (float)waves);
     const float cost = stream + (n > 1 ? 2.f * loops * std::ceil((float)n / 16.f) : 0.f);
     if (best.waves != 0 && cost >= least) return;
     least = cost;
-    best.waves = waves;
-    best.heads = heads;
-    best.shares = shares;
+    best = {waves, heads, min_len, shares, 0};
   };
-  consider(4, 1, 1.7f);
-  if (n_kv % 2 == 0) consider(4, 2, 1.25f);
-  if (n_kv % 4 == 0) consider(4, 4, 1.f);
-  if (n_kv % 8 == 0 && head_dim == 128 && cols <= 32) consider(8, 8, 0.93f);  // (with more columns 8 waves' accumulators are no room for)
+  for (int min_len = 128; min_len <= (cols <= 16 ? 128 : 1024); min_len *= 2) {
+    consider(4, 1, 1.7f, min_len);
+    if (n_kv % 2 == 0) consider(4, 2, 1.25f, min_len);
+    if (n_kv % 4 == 0) consider(4, 4, 1.f, min_len);
+    if (n_kv % 8 == 0 && head_dim == 128 && cols <= 32) consider(8, 8, 0.93f, min_len);  // (with more columns 8 waves' accumulators are no room for)
+  }
   best.max_shares = best.shares + batch;
   return best;
 }
-size_t counts_bytes(int64_t batch, int64_t n_kv) { return (size_t)(batch * n_kv) * kCountWords * sizeof(unsigned long long); }
+size_t counts_bytes(int64_t batch, int64_t n_kv, int64_t blocks) { return (size_t)(blocks * batch * n_kv) * kCountWords * sizeof(unsigned long long); }
 
 }  // namespace
 
-int64_t mxfp4_max_columns(int64_t head_dim) { return head_dim == 128 ? 64 : 32; }
+// Short query blocks: those in few enough blocks of queries, each of which reads and converts the keys again, that unpacking them for the 16-bit pool's
+// kernels takes longer.  32 requests of 4 K keys of 8 heads, 8 q heads each, us with the codes read and unpacked: 16 queries (2 blocks) 168 and 305, 24 (3)
+// 274 and 319, 32 (4) 320 and 336, 8 of 2 K 52 and 50; 2 heads of 256: 8 queries (2) 57 and 153, 16 (4) 95 and 165, 32 (8) 168 and 202, 8 of 4 K 48 and 52.
+bool mxfp4_reads_codes(int64_t group, int64_t head_dim, int64_t max_len_extend) {
+  const QueryBlocks q(group, head_dim, max_len_extend);
+  return q.cols <= most_columns(head_dim) && q.blocks <= (head_dim == 128 ? 3 : 8);
+}
 
 // For every plan: which one it is may depend on a window
 size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend) {
-  const int64_t cols = n_q / n_kv * max_len_extend, most = device_cus() + batch;
-  return counts_bytes(batch, n_kv) + (size_t)(most * n_kv * cols) * (size_t)(head_dim + 1) * sizeof(float);
+  const QueryBlocks q(n_q / n_kv, head_dim, max_len_extend);
+  const int64_t most = device_cus() + batch;
+  return counts_bytes(batch, n_kv, q.blocks) + (size_t)(q.blocks * most * n_kv * q.cols) * (size_t)(head_dim + 1) * sizeof(float);
 }
 
 int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
-  const int64_t n_kv = a.pool.n_kv, d = a.pool.head_dim, cols = a.n_q / n_kv * a.max_len_extend;
-  if (cols < 1 || cols > mxfp4_max_columns(d)) return MSGL_ERR_SHAPE;
+  const int64_t n_kv = a.pool.n_kv, d = a.pool.head_dim;
+  const QueryBlocks q(a.n_q / n_kv, d, a.max_len_extend);
+  const int64_t cols = q.cols;
+  if (cols < 1 || cols > most_columns(d) || q.blocks > 65535) return MSGL_ERR_SHAPE;
   if (a.f16 && cols > 16) return MSGL_ERR_DTYPE;
-  const int64_t keys = visible_keys(a.batch, a.total_kv, a.window, a.max_len_extend, a.is_cross != 0);
-  const Plan plan = plan_of(a.batch, keys, n_kv, d, cols);
+  const int64_t keys = visible_keys(a.batch, a.total_kv, a.window, q.queries, a.is_cross != 0);
+  const Plan plan = plan_of(a.batch, keys, n_kv, d, q);
   ShareParams p{};
   p.q = static_cast<const uint16_t*>(a.q);
   p.k_cache = static_cast<const uint16_t*>(a.pool.codes);  // as bytes, strides too
@@ -412,7 +434,8 @@ int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   p.group = (int32_t)(a.n_q / n_kv);
   p.per_group = 65535u / (uint32_t)p.group + 1u;
   p.cols = (int32_t)cols;
-  p.max_len_extend = p.q_cap = a.max_len_extend;
+  p.max_len_extend = (int32_t)q.queries;
+  p.q_cap = a.max_len_extend;
   p.f16 = a.f16;
   p.is_cross = a.is_cross;
   p.window = a.window;
@@ -428,19 +451,20 @@ int launch_mxfp4_attention(const Mxfp4AttentionArgs& a, hipStream_t stream) {
   p.min_len = (float)plan.min_len;
   p.wave_shift = __builtin_ctz((unsigned)(plan.waves / plan.heads));
   p.counts = static_cast<unsigned long long*>(a.workspace);
-  p.part_o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + counts_bytes(a.batch, n_kv));
-  p.part_lse = p.part_o + (size_t)plan.max_shares * (size_t)(n_kv * cols) * (size_t)d;
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + counts_bytes(a.batch, n_kv, q.blocks));
+  p.part_lse = p.part_o + (size_t)(plan.max_shares * q.blocks) * (size_t)(n_kv * cols) * (size_t)d;
   p.nonce = next_launch_number();
   const int64_t units = plan.max_shares * p.head_groups;
   if (units > 0x7fffffffLL) return MSGL_ERR_SHAPE;
+  const dim3 grid((unsigned)units, (unsigned)q.blocks);
   const int nct = (int)((cols + 15) / 16);
   auto launch = [&](auto dim, auto tiles, auto half) {
     constexpr int D = decltype(dim)::value, NCT = decltype(tiles)::value;
     constexpr bool F16 = decltype(half)::value;
     if constexpr (D == 128 && NCT <= 2) {
-      if (plan.waves == 8) return launch_walk<D, NCT, 8, F16>(p, units, stream);
+      if (plan.waves == 8) return launch_walk<D, NCT, 8, F16>(p, grid, stream);
     }
-    return launch_walk<D, NCT, 4, F16>(p, units, stream);
+    return launch_walk<D, NCT, 4, F16>(p, grid, stream);
   };
   using std::integral_constant;
   if (d == 128) {
