@@ -219,3 +219,73 @@ def test_same_bits_every_time(gpu):
     a = _decode(gpu, [900, 40, 2000], 8, 4, 128)
     for _ in range(3):
         assert torch.equal(a, _decode(gpu, [900, 40, 2000], 8, 4, 128))
+
+
+# launches whose requests are cut in every way: one head, two, four or eight to a workgroup, more requests than workgroups, more than stay in registers, one
+# request alone with as many shares as there are, partials of more shares than one trip of the merge takes
+CUTS = [([2000] * 40 + [37, 0, 4000] * 8, 32, 8, 128), ([300, 1, 900] * 90, 8, 8, 128), ([10] * 260 + [3000, 0, 0, 700], 8, 2, 128), ([0] * 300 + [5], 4, 1, 128),
+        ([30000], 32, 8, 128), ([20000, 1], 4, 1, 128), ([9000, 200, 4000, 1, 5000], 16, 16, 128), ([1500] * 12, 12, 4, 256), ([16000], 16, 2, 256),
+        ([700 + 97 * i for i in range(30)], 10, 5, 256), ([1200 + 31 * i for i in range(66)], 16, 8, 128)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lens,n_q,n_kv,d", CUTS)
+def test_decode_cuts(gpu, lens, n_q, n_kv, d, dtype):
+    _decode(gpu, lens, n_q, n_kv, d, dtype)
+
+
+# more columns than a workgroup's waves hold: up to three blocks of queries (eight at 256), the last of them short, and requests with nothing in the later ones
+BLOCKS = [(64, 8, 128, [9, 16, 1, 0, 24]), (32, 8, 128, [48, 1]), (8, 1, 128, [24, 5, 9, 17]), (13, 13, 128, [130, 65, 64]), (16, 2, 256, [8, 3, 5, 1]),
+          (64, 4, 256, [2, 16, 0]), (16, 2, 256, [32, 17, 1]), (4, 4, 256, [33, 200, 64]), (64, 1, 128, [1, 3, 2]), (32, 1, 256, [8, 1])]
+
+
+@pytest.mark.parametrize("is_cross,window", [(False, 0), (True, 0), (False, 1), (False, 50), (True, 50)])
+@pytest.mark.parametrize("n_q,n_kv,d,new", BLOCKS)
+def test_extend_blocks_of_queries(gpu, n_q, n_kv, d, new, is_cross, window):
+    from mini_sglang_amd_kernel import paged_prefill_attention_mxfp4
+
+    cached = [(377 * i * i + 900) % 1601 for i in range(len(new))]
+    lens = [c + e for c, e in zip(cached, new)]
+    codes, scales = pool(sum(lens) + 1, n_kv, d, 3)
+    idx, q = listed(lens, sum(lens) + 1, 4), rows(sum(new), n_q, d, 5)
+    qo, ip, prefix = indptr(new), indptr(lens), torch.tensor(cached, dtype=torch.int32)
+    got = paged_prefill_attention_mxfp4(q.to(gpu), codes.to(gpu), scales.to(gpu), qo.to(gpu), ip.to(gpu), idx.to(gpu), prefix.to(gpu), d ** -0.5,
+                                        max(new), is_cross_attention=is_cross, sliding_window_size=window)
+    out, spread, score = mx.attention(q, codes, scales, qo, ip, idx, prefix, d ** -0.5, is_cross=is_cross, window=window)
+    assert_within(got, out, spread, tolerance(spread, score, out, d), f"{n_q}/{n_kv} x {d}, {new} on {cached}")
+
+
+def test_extend_long_prefixes_of_many_shares(gpu):
+    """Partials of wide launches: 64 columns and 32 of 256, four, eight and more shares to a request."""
+    for n_q, n_kv, d, new, cached in ((32, 8, 128, [16, 2], [9000, 300]), (32, 8, 128, [8] * 5, [5000, 1, 900, 2500, 30]), (16, 2, 256, [4], [20000]),
+                                      (16, 2, 256, [8, 8], [6000, 7000]), (64, 8, 128, [3] * 40, [500 + 60 * i for i in range(40)])):
+        _extend(gpu, n_q, n_kv, d, new, cached, False, 0)
+
+
+def test_scale_of_zero(gpu):
+    """The mean of the visible values, infinite scores or none."""
+    from mini_sglang_amd_kernel import paged_decode_attention_mxfp4, paged_prefill_attention_mxfp4
+
+    lens, n_q, n_kv, d = [40, 0, 900, 1], 8, 2, 128
+    codes, scales = pool(sum(lens), n_kv, d, 1)
+    idx, ip, q = listed(lens, sum(lens), 2), indptr(lens), rows(4, n_q, d, 3)
+    q[0] = math.inf
+    got = paged_decode_attention_mxfp4(q.to(gpu), codes.to(gpu), scales.to(gpu), ip.to(gpu), idx.to(gpu), 0.0)
+    out, spread, score = mx.attention(torch.zeros_like(q), codes, scales, None, ip, idx, None, 1.0)
+    assert_within(got, out, spread, tolerance(spread, score, out, d))
+    qo, prefix = indptr([1, 0, 2, 1]), torch.tensor([39, 0, 898, 0], dtype=torch.int32)
+    got = paged_prefill_attention_mxfp4(q.to(gpu), codes.to(gpu), scales.to(gpu), qo.to(gpu), ip.to(gpu), idx.to(gpu), prefix.to(gpu), 0.0, 2)
+    out, spread, score = mx.attention(torch.zeros_like(q), codes, scales, qo, ip, idx, prefix, 1.0)
+    assert_within(got, out, spread, tolerance(spread, score, out, d))
+
+
+@pytest.mark.parametrize("byte", [0x00, 0xff, 0x7f, 0x01])
+def test_whatever_a_workspace_held(gpu, byte):
+    """Memory that the allocator hands out again is full of something: counts and partials of an earlier life."""
+    for lens, n_q, n_kv in (([3000, 40, 900], 16, 8), ([700] * 66, 8, 8)):
+        want = _decode(gpu, lens, n_q, n_kv, 128)
+        torch.cuda.synchronize()
+        for size in (1 << 16, 1 << 20, 1 << 21, 1 << 22, 1 << 23, 1 << 24, 1 << 25):
+            junk = [torch.full((size,), byte, dtype=torch.uint8, device=gpu) for _ in range(3)]
+            del junk
+        assert torch.equal(want, _decode(gpu, lens, n_q, n_kv, 128))
