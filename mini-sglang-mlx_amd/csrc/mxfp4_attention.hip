@@ -358,14 +358,16 @@ struct Plan {
 };
 // Which of them, by what a launch takes for each, in us, of the average request:
 //   bytes     at 6 TB/s with 4 heads to a workgroup, whose lines lie side by side, in 1.25 of that with 2 and 1.7 with 1; 8 waves of 8 heads, 1 KiB a slot, are
-//             faster still (16 requests of 64 K keys, 8 heads: 200 us with 8, 220 with 4, 259 with 2, 379 with 1)
-//   a wave    0.018 a key of 16 columns of 128, where there is little else (one request of 2 K keys, 4 heads 13.7, 2 10.3, 1 8.6)
-//   the merge 2 a trip of the loop in put_shares_together(), of which the more heads a workgroup has the more shares there are and the fewer threads to a head (16 of 4 K
+//             faster still; longer by the CUs that get none (16 requests of 64 K keys, 8 heads: 200 us with 8, 220 with 4, 259 with 2, 379 with 1)
+//             Two tiles of columns are bound by their arithmetic as well, and want two waves to a SIMD: 8 waves of 4 heads 0.98, of 2 1.2 (32 requests of 4 K keys, 32
+//             columns: 4 heads with 4 waves 51.1 us, with 8 48.4, 2 heads 51.5 and 49.6)
+//   a wave    0.018 a key and tile of columns, where there is little else (one request of 2 K keys, 4 heads 13.7 us, 2 10.3, 1 8.6)
+//   the merge 3, and 2 a trip of the loop in put_shares_together(), of which the more heads a workgroup has the more shares there are and the fewer threads to a head (16 of 4 K
 //             keys, 64 columns: 4 heads 91.4, 1 head 57.7; 32 columns of head_dim 256 81.7 and 35.1)
-// In 26 launches of 1 to 256 requests, 2 MB to 1.2 GB, it took the fastest of the four or one that was no more than 4 % slower.
+// Of 12 launches of 1 to 256 requests, 15 MB to 1.2 GB, that were timed in every form it takes the fastest, or one within 8 % of it.
 Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, const QueryBlocks& q) {
   const int64_t cus = device_cus(), cols = q.cols;
-  const float wave_key = 0.018f * (0.5f + 0.5f * (float)((cols + 15) / 16 * head_dim / 128));
+  const float wave_key = 0.018f * (float)((cols + 15) / 16);
   Plan best{};
   float least = 0.f;
   auto consider = [&](int waves, int heads, float rate, int min_len) {
@@ -374,8 +376,9 @@ Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, const 
     const float len = std::max(request / std::max((float)shares / (float)batch, 1.f), (float)min_len);
     const int n = std::max((int)(request / len + 0.5f), 1);
     const float loops = (float)(cols * head_dim / 4) / (float)(64 * waves / heads) / (n <= 4 ? 4.f : n <= 8 ? 2.f : 1.f);
-    const float stream = std::max((float)(keys * n_kv * head_dim * q.blocks) * (17.f / 16.f / 6e6f) * rate, wave_key * len * (float)heads / (float)waves);
-    const float cost = stream + (n > 1 ? 2.f * loops * std::ceil((float)n / 16.f) : 0.f);
+    const float idle = std::max((float)shares / (float)(n * batch), 1.f);
+    const float stream = std::max((float)(keys * n_kv * head_dim * q.blocks) * (17.f / 16.f / 6e6f) * rate * idle, wave_key * len * (float)heads / (float)waves);
+    const float cost = stream + (n > 1 ? 3.f + 2.f * loops * std::ceil((float)n / 16.f) : 0.f);
     if (best.waves != 0 && cost >= least) return;
     least = cost;
     best = {waves, heads, min_len, shares, 0};
@@ -384,7 +387,11 @@ Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, const 
     consider(4, 1, 1.7f, min_len);
     if (n_kv % 2 == 0) consider(4, 2, 1.25f, min_len);
     if (n_kv % 4 == 0) consider(4, 4, 1.f, min_len);
-    if (n_kv % 8 == 0 && head_dim == 128 && cols <= 32) consider(8, 8, 0.93f, min_len);  // (with more columns 8 waves' accumulators are no room for)
+    if (head_dim != 128 || cols > 32) continue;  // (8 waves' accumulators are no room for)
+    if (n_kv % 8 == 0) consider(8, 8, 0.93f, min_len);
+    if (cols <= 16) continue;
+    if (n_kv % 2 == 0) consider(8, 2, 1.2f, min_len);
+    if (n_kv % 4 == 0) consider(8, 4, 0.98f, min_len);
   }
   best.max_shares = best.shares + batch;
   return best;
