@@ -37,6 +37,7 @@ Unpacked unpacked(int64_t total_kv, int64_t n_kv, int64_t d) {
   const size_t rows = whole((size_t)total_kv * n_kv * d * 2);
   return Unpacked{0, rows, 2 * rows, 2 * rows + whole((size_t)total_kv * sizeof(int32_t))};
 }
+constexpr int64_t kMostKeys = (int64_t)1 << 30;  // listed: a wave's place among a share's ids is 32 bits of bytes
 bool reads_pool(int64_t n_q, int64_t n_kv, int64_t d, int64_t max_len_extend) { return msgl::mxfp4_reads_codes(n_q / n_kv, d, max_len_extend); }
 
 }  // namespace
@@ -132,7 +133,7 @@ int msgl_paged_decode_attention_mxfp4(const void* q, const void* kv_codes, const
                                       int64_t total_kv, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
                                       int64_t num_slots, int64_t codes_stride0, int64_t scales_stride0, float sm_scale, int32_t dtype,
                                       void* stream) {
-  if (batch < 0 || total_kv < 0 || batch > 0x7fffffffLL || total_kv > 0x7fffffffLL) return MSGL_ERR_SHAPE;
+  if (batch < 0 || total_kv < 0 || batch > 0x7fffffffLL || total_kv > kMostKeys) return MSGL_ERR_SHAPE;
   if (const int rc = check_sizes(num_kv_heads, head_dim, num_slots, codes_stride0, scales_stride0)) return rc;
   if (const int rc = check_heads(num_q_heads, num_kv_heads)) return rc;
   if (num_q_heads / num_kv_heads > 16) return MSGL_ERR_GROUP_TOO_LARGE;
@@ -179,7 +180,7 @@ int msgl_paged_prefill_attention_mxfp4(const void* q, const void* kv_codes, cons
   if (const int rc = check_heads(num_q_heads, num_kv_heads)) return rc;
   if (sliding_window_size < 0) return MSGL_ERR_WINDOW;
   if (batch <= 0) return MSGL_ERR_BATCH;
-  if (total_q < 0 || total_kv < 0 || batch > 0x7fffffffLL || total_q > 0x7fffffffLL || total_kv > 0x7fffffffLL) return MSGL_ERR_SHAPE;
+  if (total_q < 0 || total_kv < 0 || batch > 0x7fffffffLL || total_q > 0x7fffffffLL || total_kv > kMostKeys) return MSGL_ERR_SHAPE;
   if (const int rc = check_dtype(dtype, false)) return rc;
   if (total_q == 0 || max_len_extend <= 0) return MSGL_OK;
   const Mxfp4Pool pool = pool_of(kv_codes, kv_scales, codes_stride0, scales_stride0, num_slots, num_kv_heads, head_dim);

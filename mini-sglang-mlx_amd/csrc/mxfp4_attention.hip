@@ -33,9 +33,8 @@ struct MxShare {
 };
 // How requests are cut: the shortest length of a share, min_len at least, with which there are no more shares than fit on the card at once.  It is between
 // total / shares and what is enough when every request loses a whole share to its end, and the wave that wants to know looks for it there: 64 requests at a
-// time, which stay in registers up to kCached of them.  (Beyond those, and where even a share to a request is too many, the outer end is taken.)
+// time, which stay in registers up to kCached of them.  (Beyond those the outer end is taken.)  Where even a share to a request is too many, each has one.
 constexpr int kCached = 256;
-constexpr float kOneShare = 0x1p31f;  // keys, no request has more
 // (The quotient of floats may take an exact one a share too far, never two; `max_shares` of the launch has room for a share more of every request that has keys.)
 __device__ __forceinline__ int shares_of(int visible, float per_len) { return (int)ceilf((float)visible * per_len); }
 
@@ -56,10 +55,15 @@ __device__ __forceinline__ bool find_mx_share(const ShareParams& p, int item, Mx
     total += wave_sum(visible[c]);
     some += __popcll(__ballot(visible[c] > 0));
   }
-  for (int b0 = kCached; b0 < p.batch; b0 += kWave) {
+  for (int b0 = kCached; b0 < p.batch && some < p.shares; b0 += kWave) {
     const int n = visible_of(request_at(b0), b0);
     total += wave_sum(n);
     some += __popcll(__ballot(n > 0));
+  }
+  if (some >= p.shares) {
+    if (item >= p.batch) return false;
+    *x = {request_info(p, item), item, 0, 1, (int)(blockIdx.y * (gridDim.x / p.head_groups)) + item};
+    return true;
   }
   auto fit = [&](float len) {
     const float per_len = __builtin_amdgcn_rcpf(len);
@@ -70,8 +74,8 @@ __device__ __forceinline__ bool find_mx_share(const ShareParams& p, int item, Mx
     return wave_sum(n) <= p.shares;
   };
   float len = fmaxf((float)total * __builtin_amdgcn_rcpf((float)p.shares), p.min_len);  // from here ..
-  float most = some < p.shares ? fmaxf((float)total * __builtin_amdgcn_rcpf((float)(p.shares - some)), p.min_len) : kOneShare;  // .. to here
-  if (some >= p.shares || p.batch > kCached) {
+  float most = fmaxf((float)total * __builtin_amdgcn_rcpf((float)(p.shares - some)), p.min_len);  // .. to here
+  if (p.batch > kCached) {
     len = most;
   } else if (!fit(len)) {
     while (most > len * (1.f + 1.f / 32)) {

@@ -223,7 +223,7 @@ def test_same_bits_every_time(gpu):
 
 # launches whose requests are cut in every way: one head, two, four or eight to a workgroup, more requests than workgroups, more than stay in registers, one
 # request alone with as many shares as there are, partials of more shares than one trip of the merge takes
-CUTS = [([2000] * 40 + [37, 0, 4000] * 8, 32, 8, 128), ([300, 1, 900] * 90, 8, 8, 128), ([10] * 260 + [3000, 0, 0, 700], 8, 2, 128), ([0] * 300 + [5], 4, 1, 128),
+CUTS = [([2000] * 40 + [37, 0, 4000] * 8, 32, 8, 128), ([300, 1, 900] * 90, 8, 8, 128), ([10] * 260 + [3000, 0, 0, 700], 8, 2, 128), ([0] * 300 + [5], 4, 1, 128), ([3, 0, 1, 40] * 300 + [2000, 0], 2, 2, 128), ([0] * 500 + [90, 1] * 200 + [0, 70], 4, 4, 256),
         ([30000], 32, 8, 128), ([20000, 1], 4, 1, 128), ([9000, 200, 4000, 1, 5000], 16, 16, 128), ([1500] * 12, 12, 4, 256), ([16000], 16, 2, 256),
         ([700 + 97 * i for i in range(30)], 10, 5, 256), ([1200 + 31 * i for i in range(66)], 16, 8, 128)]
 

@@ -152,7 +152,7 @@ def test_c_entries_refuse_before_any_launch():
                                                      0.1, dtype, None)
 
     assert dec(d=64) == -2 and dec(n_q=7) == -3 and dec(n_q=34) == -4 and dec(dtype=2) == -5 and dec(ws=None) == -8 and dec(size=64) == -8
-    assert dec(q=None) == -1 and dec(idx=None) == -1 and dec(q=odd) == -10 and dec(batch=-1) == -9 and dec(total=1 << 31) == -9 and dec(batch=0) == 0
+    assert dec(q=None) == -1 and dec(idx=None) == -1 and dec(q=odd) == -10 and dec(batch=-1) == -9 and dec(total=1 << 31) == -9 and dec(total=(1 << 30) + 1) == -9 and dec(batch=0) == 0
 
     def pre(q=fake, ws=fake, size=1 << 45, batch=2, total_q=9, total=100, n_q=8, d=128, most=5, window=0, dtype=0, pl=fake):
         return lib.msgl_paged_prefill_attention_mxfp4(q, fake, fake, fake, fake, fake, pl, fake, ws, size, batch, total_q, total, n_q, 2, d, 8, 2 * d,
