@@ -34,7 +34,7 @@ struct MxShare {
 // How requests are cut: the shortest length of a share, min_len at least, with which there are no more shares than fit on the card at once.  It is between
 // total / shares and what is enough when every request loses a whole share to its end, and the wave that wants to know looks for it there: 64 requests at a
 // time, which stay in registers up to kCached of them.  (Beyond those the outer end is taken.)  Where even a share to a request is too many, each has one.
-constexpr int kCached = 256;
+constexpr int kCached = 512;
 // (The quotient of floats may take an exact one a share too far, never two; `max_shares` of the launch has room for a share more of every request that has keys.)
 __device__ __forceinline__ int shares_of(int visible, float per_len) { return (int)ceilf((float)visible * per_len); }
 
@@ -360,6 +360,10 @@ struct Plan {
   int waves, heads, min_len;
   int64_t shares, max_shares;
 };
+int64_t shares_at_once(int64_t batch, int64_t n_kv, int heads, int64_t blocks, bool two_to_a_cu) {
+  const int64_t shares = std::max<int64_t>(device_cus() / (n_kv / heads * blocks), 1);
+  return two_to_a_cu && batch > shares ? 2 * shares : shares;
+}
 // Which of them, by what a launch takes for each, in us, of the average request:
 //   bytes     at 6 TB/s with 4 heads to a workgroup, whose lines lie side by side, in 1.25 of that with 2 and 1.7 with 1; 8 waves of 8 heads, 1 KiB a slot, are
 //             faster still; longer by the CUs that get none (16 requests of 64 K keys, 8 heads: 200 us with 8, 220 with 4, 259 with 2, 379 with 1)
@@ -370,18 +374,22 @@ struct Plan {
 //             keys, 64 columns: 4 heads 91.4, 1 head 57.7; 32 columns of head_dim 256 81.7 and 35.1)
 // Of 12 launches of 1 to 256 requests, 15 MB to 1.2 GB, that were timed in every form it takes the fastest, or one within 8 % of it.
 Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, const QueryBlocks& q) {
-  const int64_t cus = device_cus(), cols = q.cols;
+  const int64_t cols = q.cols;
   const float wave_key = 0.018f * (float)((cols + 15) / 16);
+  // More requests than CUs for them: two workgroups to a CU, so that the longest can be cut (300 requests of 500-1500 keys, 8 heads: 109.7 and 79.0 us).  Where a
+  // CU has a share for every request it takes one (256 of 1-3 K: 119 and 133).
+  const bool one_tile = cols <= 16 && head_dim == 128, two_tiles = cols <= (head_dim == 128 ? 32 : 16);  // LDS and registers for 16 and for 8 waves
   Plan best{};
   float least = 0.f;
   auto consider = [&](int waves, int heads, float rate, int min_len) {
-    const int64_t shares = std::max<int64_t>(cus / (n_kv / heads * q.blocks), 1);
+    const int64_t shares = shares_at_once(batch, n_kv, heads, q.blocks, one_tile || (two_tiles && waves == 4));
     const float request = (float)keys / (float)batch;
     const float len = std::max(request / std::max((float)shares / (float)batch, 1.f), (float)min_len);
     const int n = std::max((int)(request / len + 0.5f), 1);
     const float loops = (float)(cols * head_dim / 4) / (float)(64 * waves / heads) / (n <= 4 ? 4.f : n <= 8 ? 2.f : 1.f);
     const float idle = std::max((float)shares / (float)(n * batch), 1.f);
-    const float stream = std::max((float)(keys * n_kv * head_dim * q.blocks) * (17.f / 16.f / 6e6f) * rate * idle, wave_key * len * (float)heads / (float)waves);
+    const float uneven = shares <= batch ? 1.15f : 1.f;  // nothing is cut: the longest request decides
+    const float stream = std::max((float)(keys * n_kv * head_dim * q.blocks) * (17.f / 16.f / 6e6f) * rate * idle * uneven, wave_key * len * (float)heads / (float)waves);
     const float cost = stream + (n > 1 ? 3.f + 2.f * loops * std::ceil((float)n / 16.f) : 0.f);
     if (best.waves != 0 && cost >= least) return;
     least = cost;
@@ -415,7 +423,9 @@ bool mxfp4_reads_codes(int64_t group, int64_t head_dim, int64_t max_len_extend) 
 // For every plan: which one it is may depend on a window
 size_t mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len_extend) {
   const QueryBlocks q(n_q / n_kv, head_dim, max_len_extend);
-  const int64_t most = device_cus() + batch;
+  int64_t most = 0;
+  for (int heads = 1; heads <= (q.cols <= 32 ? 8 : 4) && n_kv % heads == 0; heads *= 2) most = std::max(most, shares_at_once(batch, n_kv, heads, q.blocks, true));
+  most += batch;
   return counts_bytes(batch, n_kv, q.blocks) + (size_t)(q.blocks * most * n_kv * q.cols) * (size_t)(head_dim + 1) * sizeof(float);
 }
 
