@@ -46,12 +46,12 @@ struct MxTile {  // 32 keys as they lie in the pool
 };
 
 // The factor of a block as the conversion wants it.  Half reaches 65504 = 2^16 (1 - 2^-11) while a block that holds that much has the unit 2^14 and codes up to
-// 6: K and V come in at half their size there, and scores and results are doubled.
+// 6: K and V come in at half their size there, and scores and results are doubled.  Byte 0, of a slot that nobody stored, stays 0: its codes are zeros.
 template <bool F16, bool IS_K>
 __device__ __forceinline__ float block_factor(uint32_t byte) {
   if constexpr (!F16) return mx_scale(byte);
-  else if constexpr (IS_K) return mx_scale(byte == kMxNotFinite ? byte : byte - 1);
-  else return mx_scale(byte - 1);
+  else if constexpr (IS_K) return mx_scale(byte == kMxNotFinite ? byte : max(byte, 1u) - 1);
+  else return mx_scale(max(byte, 1u) - 1);
 }
 template <bool F16>
 constexpr float kBack = F16 ? 2.f : 1.f;
