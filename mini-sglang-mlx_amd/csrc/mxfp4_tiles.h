@@ -14,7 +14,7 @@
 //                  weights of group g's keys are the ones that its lanes hold.
 // The conversion multiplies by the block's factor on the way (one instruction for two values), so codes cost what 16-bit values would.
 // Weights are rounded to the type of q for the second product (half a step, 2^-8 and 2^-11 of a weight, as the 16-bit pool's
-// kernels do); scores, sums and accumulators have 32 bits, and so do the partials.
+// kernels do; for what half does not reach see kLift); scores, sums and accumulators have 32 bits, and so do the partials.
 #pragma once
 #include <type_traits>
 
@@ -33,8 +33,8 @@ struct MxColumns {
   u32x4_t q[NCT][D / 32];      // [4 h + c]: dims 128 h + 32 g + 8 c ..
   int lo[NCT], hi[NCT];        // first and last visible key of this lane's column in each tile of 16
   int all_lo, all_hi;          // keys inside are visible to every column
-  float m[NCT], l[NCT];        // what the weights are relative to (base 2; 0 before the first key); this lane's part of their sum
-  float top[NCT];              // m, or -infinity before the first key
+  float m[NCT], l[NCT];        // the reference of the weights (base 2; 0 before the first key) less kLift; this lane's part of their sum
+  float top[NCT];              // the reference, or -infinity before the first key
   f32x4_t o[NCT][D / 128][8];  // [h][n][i]: dim 128 h + 8 (4 g + i) + n
 };
 
@@ -55,6 +55,14 @@ __device__ __forceinline__ float block_factor(uint32_t byte) {
 }
 template <bool F16>
 constexpr float kBack = F16 ? 2.f : 1.f;
+
+// Weights are 2^(kLift + score - reference), and the reference moves where a score is more than kReach above it.  Half holds 11 bits of a number from 2^-14 on,
+// steps of 2^-24 below, and 65504: from 2^13 to 2^15 for the largest weight of a wave's keys, the others keep their 11 bits down to 2^-27 of it, and
+// are off by at most 2^-38 of it below.  (At 1, as in bf16, which has the range, a key 17 above all others in the exponent left nothing of them.)
+template <bool F16>
+constexpr float kLift = F16 ? 13.f : 0.f;
+template <bool F16>
+constexpr float kReach = F16 ? 2.f : kLazy;
 
 template <int D, int NCT, bool F16>
 __device__ __forceinline__ void start_mx_columns(const MxParams& p, const ReqInfo& r, int kvh, int t_end, MxColumns<D, NCT>& c_) {
@@ -183,13 +191,13 @@ __device__ __forceinline__ void compute_mx_tile(const SplitKvParams& p, const Mx
       }
     }
     const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * p.scale_log2e;
-    // The reference moves only where a score is far beyond it: weights up to 2^kLazy are as exact as those up to 1
-    if (__any(mx > c_.top[ct] + kLazy)) {
+    // The reference moves only where a score is far beyond it: weights up to 2^kReach are as exact as those up to 1
+    if (__any(mx > c_.top[ct] + kReach<F16>)) {
       const float top = fmaxf(c_.top[ct], max_across<32>(max_across<16>(mx)));
       const float m = top == kNegInf ? 0.f : top;
       const float alpha = fast_exp2(c_.top[ct] - m);
       c_.top[ct] = top;
-      c_.m[ct] = m;
+      c_.m[ct] = m - kLift<F16>;
       c_.l[ct] *= alpha;
 #pragma unroll
       for (int h = 0; h < D / 128; ++h)

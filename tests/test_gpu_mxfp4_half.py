@@ -37,3 +37,27 @@ def test_slots_that_nobody_stored(gpu, d, dtype):
     out, spread, score = mx.attention(q, codes, scales, None, ip, inside, None, d ** -0.5)
     assert (got[[0, 3, 4]] == 0).all() and (out[[0, 3, 4]] == 0).all()
     assert_within(got, out, spread, tolerance(spread, score, out, d, dtype))
+
+
+def _bound(spread, score, out, d, largest, n=0):
+    """As `tolerance` of half, with what half's range costs as it is: a weight is off by 2^-11 of itself or 2^-38 of the largest (`largest`: of
+    the values that meet them, for `n` keys), a value by 2^-24, half of the step of V at half its size, and the result by half a step of its own, 2^-25 at the least."""
+    half_step = 2.0 ** -11
+    return (half_step * (1 + 2.0 ** -6) * (spread + out.abs()) + (half_step * out.abs()).clamp_min(2.0 ** -25) * (1 + half_step * 4) + n * 2.0 ** -37 * largest
+            + 2.0 ** -24 + spread * (2 * (d + 2) * 2.0 ** -24 * score[..., None] + 2.0 ** -18))
+
+
+@pytest.mark.parametrize("batch", [1, 600])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("n,above", [(2, 18), (33, 18), (700, 18), (2, 23), (700, 23)])
+def test_weights_beside_one_that_is_far_larger(gpu, n, above, d, batch):
+    """A key this much above the others in the exponent, whose V is zero: what is left is all of the others'.  600 requests, whose keys nobody cuts, and one."""
+    k, v = torch.zeros(n, 2, d, dtype=F16), rows(n, 2, d, 1, F16, 2.0 ** 13)
+    k[n // 2], v[n // 2] = 2.0, 0.0
+    codes, scales = mx.quantised(k, v)
+    q, idx, scale = torch.ones(1, 8, d, dtype=F16), torch.arange(n, dtype=torch.int32), above / (2 * d)
+    out, spread, score = mx.attention(q, codes, scales, None, indptr([n]), idx, None, scale)
+    assert float(score.max()) == above and float(out.abs().max()) > 2.0 ** -20
+    got = _decode(gpu, q.expand(batch, 8, d), codes, scales, indptr([n] * batch), idx.repeat(batch), scale)
+    assert torch.equal(got, got[:1].expand(batch, 8, d))
+    assert_within(got[:1], out, spread, _bound(spread, score, out, d, float(v.abs().max()) * 4 / 3, n))
