@@ -13,7 +13,7 @@
  * The reference has no such pool; the conventions are those of msgl_paged_attention.h: device pointers, nothing
  * allocated, retained or synchronised, errors as MSGL_ERR_* codes, slot ids outside the pool written nowhere by the writers and
  * clamped to the pool by the readers.  `codes_stride0` and `scales_stride0` are the BYTES from one slot to the next (the rest is
- * contiguous): multiples of 16 and of 8.  head_dim is 128 or 256.
+ * contiguous): multiples of 16 and of 8, below 2^32 (MSGL_ERR_SHAPE).  head_dim is 128 or 256.
  */
 #ifndef MSGL_MXFP4_CACHE_H
 #define MSGL_MXFP4_CACHE_H

@@ -16,6 +16,7 @@ int check_sizes(int64_t n_kv, int64_t d, int64_t num_slots, int64_t codes_stride
   if (d != 128 && d != 256) return MSGL_ERR_HEAD_DIM;
   if (n_kv <= 0 || n_kv > (1 << 20) || num_slots <= 0 || num_slots > 0x80000000ll) return MSGL_ERR_SHAPE;
   if (codes_stride0 < n_kv * d || scales_stride0 < n_kv * (d / 16)) return MSGL_ERR_SHAPE;
+  if (codes_stride0 > 0xffffffffll || scales_stride0 > 0xffffffffll) return MSGL_ERR_SHAPE;  // of 32 bits in the attention's walk
   return MSGL_OK;
 }
 int check_pool(const Mxfp4Pool& pool) {

@@ -780,6 +780,8 @@ Wrong mxfp4_pool(const Tensor& codes, const Tensor& scales, int64_t n_kv, int64_
   for (const Tensor* t : {&codes, &scales})
     if (t->stride(3) != 1 || t->stride(2) != t->size(3) || t->stride(1) != 2 * t->size(3))
       return "kv_codes and kv_scales must be contiguous behind their first dimension";
+  for (const Tensor* t : {&codes, &scales})
+    if (t->size(0) > 1 && t->stride(0) > 0xffffffffll) return "pages of kv_codes and kv_scales must lie less than 4 GiB apart";
   return {};
 }
 int64_t page_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2) * t.size(3); }
