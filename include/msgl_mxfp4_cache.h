@@ -48,7 +48,7 @@ MSGL_API int msgl_qk_norm_rope_store_mxfp4(const void* q, const void* k, const v
 
 /* One query per request over the slots listed for it: the counterpart of msgl_paged_decode_attention.  q and out
  * (batch, num_q_heads, head_dim) contiguous, bf16 or half; at most 16 q heads to a kv head.  A request without keys gets zeros.
- * total_kv is the length of kv_indices, at least kv_indptr[batch] and, for both kinds of attention, at most 2^30. */
+ * total_kv is the length of kv_indices, at least kv_indptr[batch].  Both kinds of attention take total_kv up to 2^30 and up to 2^15 kv heads. */
 MSGL_API size_t msgl_paged_decode_mxfp4_workspace_bytes(int64_t batch, int64_t total_kv, int64_t num_q_heads,
                                                         int64_t num_kv_heads, int64_t head_dim);
 MSGL_API int msgl_paged_decode_attention_mxfp4(const void* q, const void* kv_codes, const void* kv_scales,

@@ -27,7 +27,13 @@ int check_pool(const Mxfp4Pool& pool) {
 Mxfp4Pool pool_of(const void* codes, const void* scales, int64_t codes_stride0, int64_t scales_stride0, int64_t num_slots, int64_t n_kv, int64_t d) {
   return Mxfp4Pool{const_cast<void*>(codes), const_cast<void*>(scales), codes_stride0, scales_stride0, num_slots, n_kv, d};
 }
-int check_heads(int64_t n_q, int64_t n_kv) { return n_q <= 0 ? MSGL_ERR_SHAPE : n_q % n_kv != 0 ? MSGL_ERR_HEAD_RATIO : MSGL_OK; }
+// Of attention: the partials of a request, which a share's workgroup addresses by 32 bits, are at most 32 KiB a kv head and share, and there are
+// at most 4096 + 2 n_kv of those.
+constexpr int64_t kMostKvHeads = 1 << 15;
+int check_heads(int64_t n_q, int64_t n_kv) {
+  if (n_q <= 0 || n_kv > kMostKvHeads) return MSGL_ERR_SHAPE;
+  return n_q % n_kv != 0 ? MSGL_ERR_HEAD_RATIO : MSGL_OK;
+}
 
 // The unpacked rows of a prefill call, in front of the tile kernels' own workspace.
 struct Unpacked {

@@ -40,3 +40,18 @@ def test_slots_four_gib_apart_are_refused_with_the_reason():
             load_kv_cache_mxfp4(c, s, ids)
         with pytest.raises(RuntimeError, match="less than 4 GiB apart"):
             paged_decode_attention_mxfp4(torch.zeros(1, 4, 128, dtype=BF16), c, s, ids, ids, 0.1)
+
+
+def test_more_kv_heads_than_a_requests_partials_have_room_for():
+    """A request's partials are addressed by 32 bits: the entries of attention take 2^15 kv heads at most."""
+    from mini_sglang_amd_kernel import _lib
+
+    lib, f = _lib.load(), FAKE
+    for n_kv, group in (((1 << 15) + 1, 1), (1 << 17, 16), (1 << 20, 2)):
+        n_q = n_kv * group
+        for d in (128, 256):
+            size = 1 << 60
+            assert lib.msgl_paged_decode_attention_mxfp4(f, f, f, f, f, f, f, size, 2, 100, n_q, n_kv, d, 8, n_kv * d, n_kv * d // 16, 0.1, 0, None) == SHAPE
+            for most in (2, 500):
+                assert lib.msgl_paged_prefill_attention_mxfp4(f, f, f, f, f, f, f, f, f, size, 2, 9, 100, n_q, n_kv, d, 8, n_kv * d, n_kv * d // 16, 0.1, most,
+                                                              0, 0, 0, None) == SHAPE
