@@ -180,6 +180,7 @@ class AttnBackend:
             if out is not None:
                 return out
         if isinstance(cache, MXFP4KVCache):
+            cache.require_rows("forward_fused_norm_rope", k, v)
             q = qk_norm_rope_store_mxfp4(q, k, v, q_norm_weight, k_norm_weight, metadata.positions, batch.out_loc,
                                          cache.codes(layer_id), cache.scales(layer_id), eps=rms_norm_eps, rope_base=rope_base)
             return self._attend_mxfp4(q, layer_id, metadata, is_cross_attention, sliding_window_size)

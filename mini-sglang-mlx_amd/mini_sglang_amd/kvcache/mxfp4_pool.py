@@ -44,6 +44,11 @@ class MXFP4KVCache(BaseKVCache):
         """A layer's ``(num_pages, num_kv_heads, 2, head_dim / 32)`` block bytes."""
         return self._scale_layers[index]
 
+    def require_rows(self, op: str, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Rows of another type may hold what this pool's queries cannot: bf16 reaches beyond half."""
+        if k.dtype is not self._dtype or v.dtype is not self._dtype:
+            raise ValueError(f"{op}: k is {k.dtype} and v {v.dtype}, the cache's dtype is {self._dtype}")
+
     # ---- the surface of a pool ---------------------------------------------------------------
     def k_cache(self, index: int) -> torch.Tensor:
         """K's codes; their block bytes are ``scales(index)[:, :, 0]``."""
@@ -60,6 +65,7 @@ class MXFP4KVCache(BaseKVCache):
         if k.shape[0] != rows or v.shape[0] != rows:
             raise ValueError(f"store_kv: {rows} slot ids for k of shape {tuple(k.shape)} and v of "
                              f"shape {tuple(v.shape)}")
+        self.require_rows("store_kv", k, v)
         store_kv_cache_mxfp4(self._code_layers[layer_id], self._scale_layers[layer_id], out_loc, k, v)
 
     def load_kv(self, indices: torch.Tensor, layer_id: int) -> Tuple[torch.Tensor, torch.Tensor]:

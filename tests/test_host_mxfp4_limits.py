@@ -55,3 +55,26 @@ def test_more_kv_heads_than_a_requests_partials_have_room_for():
             for most in (2, 500):
                 assert lib.msgl_paged_prefill_attention_mxfp4(f, f, f, f, f, f, f, f, f, size, 2, 9, 100, n_q, n_kv, d, 8, n_kv * d, n_kv * d // 16, 0.1, most,
                                                               0, 0, 0, None) == SHAPE
+
+
+@pytest.mark.parametrize("pool,row", [(F16, BF16), (BF16, F16), (F16, torch.float32)])
+def test_rows_of_another_type_than_the_caches(pool, row):
+    """A cache's dtype is that of its rows: bf16 reaches values that a decode in half gives as infinities."""
+    from types import SimpleNamespace
+
+    from mini_sglang_amd.attention import AttnBackend
+    from mini_sglang_amd.kvcache import MXFP4KVCache
+
+    cache = MXFP4KVCache(num_kv_heads=2, num_layers=1, head_dim=128, num_pages=8, dtype=pool, device="cpu")
+    right, wrong, loc = torch.zeros(3, 2, 128, dtype=pool), torch.zeros(3, 2, 128, dtype=row), torch.arange(3, dtype=I32)
+    for k, v in ((wrong, wrong), (right, wrong), (wrong, right)):
+        with pytest.raises(ValueError, match="store_kv: .*the cache's dtype"):
+            cache.store_kv(k, v, loc, 0)
+    backend = AttnBackend(SimpleNamespace(head_dim=128), cache, torch.zeros(2, 8, dtype=I32))
+    with pytest.raises(ValueError, match="the cache's dtype"):
+        backend.store_kv_only(wrong, wrong, loc, 0)
+    batch = SimpleNamespace(out_loc=loc, attn_metadata=SimpleNamespace(positions=loc))
+    with pytest.raises(ValueError, match="the cache's dtype"):
+        backend.forward_fused_norm_rope(wrong, wrong, wrong, wrong[0, 0], wrong[0, 0], 0, batch, rms_norm_eps=1e-6, rope_base=1e4)
+    with pytest.raises(RuntimeError, match="ROCm GPU device"):  # rows of the right type get as far as the operator
+        cache.store_kv(right, right, loc, 0)
