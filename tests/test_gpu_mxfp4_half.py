@@ -61,3 +61,17 @@ def test_weights_beside_one_that_is_far_larger(gpu, n, above, d, batch):
     got = _decode(gpu, q.expand(batch, 8, d), codes, scales, indptr([n] * batch), idx.repeat(batch), scale)
     assert torch.equal(got, got[:1].expand(batch, 8, d))
     assert_within(got[:1], out, spread, _bound(spread, score, out, d, float(v.abs().max()) * 4 / 3, n))
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_the_lower_end_of_half(gpu, d):
+    """Half has K and V at half their size: exact where a block's unit is 2^-22 or more, else off by 2^-24 at most."""
+    q, idx, ip = rows(3, 8, d, 3, F16, 16.0), torch.arange(200, dtype=torch.int32), indptr([1, 99, 100])
+    q_sum = q.double().abs().sum(-1)[..., None]
+    for k_scale, v_scale in ((2.0 ** -12, 2.0 ** -12), (2.0 ** -19, 2.0 ** -19), (2.0 ** -22, 2.0 ** -22), (1.0, 2.0 ** -24)):
+        codes, scales = mx.quantised(rows(200, 2, d, 1, F16, k_scale), rows(200, 2, d, 2, F16, v_scale))
+        sm_scale = d ** -0.5 / 16 / k_scale
+        k_off = sm_scale * q_sum * 2.0 ** -24 * float((scales[:, :, 0] < 127 - 22).any())
+        out, spread, score = mx.attention(q, codes, scales, None, ip, idx, None, sm_scale)
+        bound = _bound(spread, score, out, d, v_scale * 8, 200) + 2 * spread * torch.expm1(k_off)
+        assert_within(_decode(gpu, q, codes, scales, ip, idx, sm_scale), out, spread, bound, f"{k_scale} {v_scale}")
