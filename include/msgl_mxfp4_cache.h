@@ -48,6 +48,8 @@ MSGL_API int msgl_qk_norm_rope_store_mxfp4(const void* q, const void* k, const v
 
 /* One query per request over the slots listed for it: the counterpart of msgl_paged_decode_attention.  q and out
  * (batch, num_q_heads, head_dim) contiguous, bf16 or half; at most 16 q heads to a kv head.  A request without keys gets zeros.
+ * With q in bf16 the pool's values are taken exactly.  Half takes them at half their size: those of blocks whose factor is below 2^-22 are off
+ * by 2^-24 at most, and values beyond 98304 are infinities.
  * total_kv is the length of kv_indices, at least kv_indptr[batch].  Both kinds of attention take total_kv up to 2^30 and up to 2^15 kv heads. */
 MSGL_API size_t msgl_paged_decode_mxfp4_workspace_bytes(int64_t batch, int64_t total_kv, int64_t num_q_heads,
                                                         int64_t num_kv_heads, int64_t head_dim);
@@ -59,7 +61,7 @@ MSGL_API int msgl_paged_decode_attention_mxfp4(const void* q, const void* kv_cod
 
 /* Several queries per request under the four masks of msgl_paged_prefill_attention, which this is the counterpart of (bf16).
  * Short query blocks read the pool as it is.  Longer ones have the listed rows unpacked into the workspace first, once for all their
- * queries (total_kv rows of K and V in bf16 at most), and go through the tile kernels of the 16-bit pool. */
+ * queries (total_kv rows of K and V in bf16 at most; total_kv * num_kv_heads below 2^31), and go through the tile kernels of the 16-bit pool. */
 MSGL_API size_t msgl_paged_prefill_mxfp4_workspace_bytes(int64_t batch, int64_t total_q, int64_t total_kv, int64_t num_q_heads,
                                                          int64_t num_kv_heads, int64_t head_dim, int64_t max_len_extend);
 MSGL_API int msgl_paged_prefill_attention_mxfp4(const void* q, const void* kv_codes, const void* kv_scales,

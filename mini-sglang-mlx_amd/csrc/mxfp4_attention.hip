@@ -7,7 +7,7 @@
 // us against 107, 8 of 4 K 18.7 against 15.5).  Partials and counts travel at agent scope; a count word carries the launch's number
 // (launch_number.h), so the workspace needs no clearing, and is left as of a launch that never happened, so a replay counts anew.
 //
-// Bound by memory: 16 requests of 32-128 K keys of 8 heads of 128, 6.3 TB/s; 64 of 512-8 K 5.5.
+// Bound by memory: 16 requests of 32-128 K keys of 8 heads of 128, 6.3 TB/s; 64 of 1-8 K 5.5.
 #include <cmath>
 #include <utility>
 
@@ -372,7 +372,7 @@ int64_t shares_at_once(int64_t batch, int64_t n_kv, int heads, int64_t blocks, b
 //   a wave    0.018 a key and tile of columns, where there is little else (one request of 2 K keys, 4 heads 13.7 us, 2 10.3, 1 8.6)
 //   the merge 3, and 2 a trip of the loop in put_shares_together(), of which the more heads a workgroup has the more shares there are and the fewer threads to a head (16 of 4 K
 //             keys, 64 columns: 4 heads 91.4, 1 head 57.7; 32 columns of head_dim 256 81.7 and 35.1)
-// Of 12 launches of 1 to 256 requests, 15 MB to 1.2 GB, that were timed in every form it takes the fastest, or one within 8 % of it.
+// Lengths count by their mean alone: what a long request among many short ones takes is not in it.
 Plan plan_of(int64_t batch, int64_t keys, int64_t n_kv, int64_t head_dim, const QueryBlocks& q) {
   const int64_t cols = q.cols;
   const float wave_key = 0.018f * (float)((cols + 15) / 16);

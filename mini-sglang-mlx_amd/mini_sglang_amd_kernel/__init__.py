@@ -378,8 +378,9 @@ def paged_decode_attention_mxfp4(q: torch.Tensor, kv_codes: torch.Tensor, kv_sca
                                  kv_indptr: torch.Tensor, kv_indices: torch.Tensor, sm_scale: float, *,
                                  stream=None, validate: Optional[bool] = None) -> torch.Tensor:
     """``paged_decode_attention`` over a pool of 4 bits: ``q (batch, n_q, d)``, bf16 or float16, at most 16 q heads to a
-    kv head.  The pool's values are taken exactly; a request without keys gets zeros.  (float16: values beyond 98304, which only
-    a pool stored from bf16 has, come out as infinities.)"""
+    kv head.  A request without keys gets zeros.  With q in bf16 the pool's values are taken exactly; with q in float16 at half their
+    size: those of blocks whose unit is below 2^-22 are off by 2^-24 at most, and values beyond 98304, which only a pool stored from bf16
+    has, come out as infinities."""
     if stream is None:
         return _native.paged_decode_attention_mxfp4(q, kv_codes, kv_scales, kv_indptr, kv_indices, sm_scale, validate)
     with _on_stream(stream, q):
